@@ -573,6 +573,80 @@ int vaesne_cat(const void* const* srcs, const int64_t* widths, int n, int64_t ou
 int vaesne_pack(const float* const* srcs, const int64_t* offs, const int64_t* ns, int count,
                 float* dst, int unpack, void* stream);
 
+/* ---- attention over packed sequences ----------------------------------------
+ * Sequences of different lengths lie one behind the other, without padding: q [total_q, Hq, D],
+ * k, v [total_k, Hkv, D] (rows of D unit-stride elements, 16-byte aligned; ts / hs = token / head
+ * stride in elements).  Sequence s holds tokens cu_q[s] .. cu_q[s+1] of q and cu_k[s] .. cu_k[s+1]
+ * of k, v; its queries are the LAST nq of its nk positions (query i stands at i + nk - nq).
+ *   S = scale q k^T + table[lut[clamp(j - i - (nk - nq), -R, R) + R], head]   (table: nullable)
+ *   causal: key j is seen iff j <= i + nk - nq;  o = softmax(S) v, 0 where nothing is seen.
+ * Query head h reads key head h / (Hq / Hkv).  type: 0 fp32, 1 bf16, 2 fp16 (every tensor but the
+ * fp32 statistics has it).  D: a multiple of 8, at most 128.
+ * q_tiles / k_tiles: {sequence, first position} of every tile of q_tile positions / k_tile keys, in
+ * any order (longest work first is fastest); vaesne_packed_attn_tiles gives q_tile and k_tile. */
+typedef struct vaesne_packed_attn {
+  int type, Hq, Hkv, D, causal, num_buckets, max_distance, nseq;
+  float scale;                       /* > 0 */
+  int max_q, max_k;                  /* longest sequence's queries / keys */
+  int q_tile, k_tile, n_q_tiles, n_k_tiles;
+  int64_t total_q, total_k;
+  const int32_t *cu_q, *cu_k, *q_tiles, *k_tiles;
+  const void *q, *k, *v;
+  int64_t q_ts, q_hs, k_ts, k_hs, v_ts, v_hs;
+  void* o;                           /* [total_q, Hq, D] dense (out; in for the backward) */
+  float* lse;                        /* [total_q, Hq], log2 domain, +inf where nothing is seen */
+  const void* table;                 /* [num_buckets, Hq] or null */
+  const int32_t* lut;                /* [2 max_distance + 1] buckets of the positions -R .. R */
+  const void* dout;                  /* backward: [total_q, Hq, D] */
+  int64_t do_ts, do_hs;
+  void *dq, *dk, *dv, *dtable;       /* dense, the inputs' shapes and type; dtable nullable */
+  void* workspace;                   /* vaesne_packed_attn_workspace bytes, 16-byte aligned */
+} vaesne_packed_attn;
+/* q_tile and k_tile for heads, head_dim, type, max_q and max_k of `a`. */
+int vaesne_packed_attn_tiles(const vaesne_packed_attn* a, int* q_tile, int* k_tile);
+/* Workspace bytes of the forward (backward = 0) or backward; a negative value: the sizes are refused. */
+int64_t vaesne_packed_attn_workspace(const vaesne_packed_attn* a, int backward);
+int vaesne_packed_attn_fwd(const vaesne_packed_attn* a, void* stream);
+int vaesne_packed_attn_bwd(const vaesne_packed_attn* a, void* stream);
+
+/* ---- the join between two blocks: norm, gate, residual, norm ------------------
+ *   u = N(branch) post_w (+ post_b);  y = residual_scale x + gate u;  n = N(y) pre_w (+ pre_b)
+ * over the last axis (C <= 8192), N = x / rms(x) (kind 0) or (x - mean) / std (kind 1), eps inside
+ * the root; the second norm reads y before it is rounded.  branch null: y = residual_scale x, and no
+ * post_* / gate.  gate: 0 none, 1 one per channel [C], 2 one per token and channel [rows, C].
+ * type as above, for every tensor but stats (fp32 [rows][4]: mean, 1 / std of branch and of y).
+ * ld*: row strides in elements.  Backward: dy / dn nullable (zero); dx, dbranch, dgate (gate 2) are
+ * dense; parameter gradients are fixed-order sums over the rows, each nullable. */
+typedef struct vaesne_gated_norm {
+  int type, kind, gate_kind, C;
+  int64_t rows;
+  float residual_scale, eps;
+  const void *x, *branch, *gate, *pre_w, *pre_b, *post_w, *post_b;
+  int64_t ldx, ldbranch, ldgate;
+  void *y, *n;                       /* dense; y nullable when branch is null */
+  float* stats;
+  const void *dy, *dn;
+  int64_t lddy, lddn;
+  void *dx, *dbranch, *dgate, *dpre_w, *dpre_b, *dpost_w, *dpost_b;
+  void* workspace;                   /* backward: vaesne_gated_norm_workspace bytes */
+} vaesne_gated_norm;
+int64_t vaesne_gated_norm_workspace(const vaesne_gated_norm* a);
+int vaesne_gated_norm_fwd(const vaesne_gated_norm* a, void* stream);
+int vaesne_gated_norm_bwd(const vaesne_gated_norm* a, void* stream);
+
+/* ---- activations kept in 8 bits -----------------------------------------------
+ * Blocks of 32 consecutive values share a power of two: exps[i] = max(exponent field of the block's
+ * largest |x|, 1), step = 2^(exps - 133), codes = round-half-even(x / step) clamped to +-127 (the
+ * error is at most step / 2, a whole step where 127 clips); exps 255 marks a block with a NaN or an
+ * infinity, which reads back as NaN.  codes: int8 [n], exps: uint8 [ceil(n / 32)].
+ * gelu8: y = GELU(x) (erf form) beside the codes; its backward reads only them:
+ *   dx = dy GELU'(kept x), and y_again (nullable) = GELU(kept x). */
+int vaesne_pack8(int type, const void* x, int64_t n, int8_t* codes, uint8_t* exps, void* stream);
+int vaesne_unpack8(int type, const int8_t* codes, const uint8_t* exps, int64_t n, void* x, void* stream);
+int vaesne_gelu8_fwd(int type, const void* x, int64_t n, void* y, int8_t* codes, uint8_t* exps, void* stream);
+int vaesne_gelu8_bwd(int type, const int8_t* codes, const uint8_t* exps, const void* dy, int64_t n, void* dx,
+                     void* y_again, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -36,7 +36,13 @@ CFLAGS = ["-O3", "-std=c++17", "-fPIC", f"--offload-arch={ARCH}", "-fvisibility=
 NO_PACKED_FP32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 FILE_FLAGS = {"attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form", "-fno-slp-vectorize"],
               "attention_sf16.hip": NO_PACKED_FP32,
-              "elementwise.hip": NO_PACKED_FP32}
+              "elementwise.hip": NO_PACKED_FP32,
+              "act8.hip": NO_PACKED_FP32,
+              "gated_norm.hip": NO_PACKED_FP32,
+              "packed_attention.hip": NO_PACKED_FP32,
+              "packed_attention_f32.hip": NO_PACKED_FP32,
+              "packed_attention_bf16.hip": NO_PACKED_FP32,
+              "packed_attention_f16.hip": NO_PACKED_FP32}
 
 
 def sources():

@@ -1,0 +1,863 @@
+// Attention over packed sequences (include/vaesne_hip.h: vaesne_packed_attn): one pass over the
+// keys with a running maximum and sum, every product on the matrix cores, for fp32, bf16 and fp16.
+//
+// Layout of the products.  All tiles are 32x32 accumulators (v_mfma_f32_32x32x16_{bf16,f16}, and
+// v_mfma_f32_32x32x2_f32 for fp32), and every one is oriented so that a lane owns one COLUMN: a
+// query in the forward and in dQ, a key in dK / dV.  The forward computes S^T = K Q^T (rows are
+// keys): a lane holds 16 scores of its own query, so the softmax needs one cross-lane exchange (lane
+// l and l ^ 32 share a query) per key tile.  The contraction of the next product runs over those
+// same rows (O^T = V^T P^T): a contraction may number its slots as it likes so long as both operands
+// agree, so the accumulator registers of P are, in order, the other operand's slots
+//     slot (half h, element j) of block t  <->  row  KC t + 8 (j / 4) + 4 h + j % 4
+// and V^T is read from the row-major LDS tile with that numbering (ds_read_b64_tr_b16 for 16-bit
+// types: 4 rows of one column per lane; four ds_read_b32 for fp32).  P never passes through LDS.
+// The backward repeats the scheme: dQ^T = K^T dS^T beside S^T and dP^T = V dO^T, and, with a key per
+// lane, dV^T = dO^T P and dK^T = Q^T dS beside S = Q K^T and dP = dO V^T.  dQ and dK / dV are two
+// kernels that each compute S and dP (seven products instead of five): no atomic sums, so
+// every gradient is bitwise reproducible.
+//
+// LDS tiles are rows of DP elements in 16-byte chunks, chunk c of row r at c ^ swz(r): both the row
+// reads (16 lanes: 16 rows of one chunk) and the transposed reads (32 lanes: 4 rows of 4 chunks)
+// then touch all 64 banks once.  Rows outside a sequence and columns past D are zero, so nothing
+// that lies behind a sequence can reach it.
+//
+// Grouped heads.  The PG query heads that share a key head are rows of one tile (row = position *
+// PG + head), so K and V are read once for all of them, and one new token fills PG rows, not one.
+// With few tiles the keys (forward, dQ) or the query rows (dK / dV) are split over workgroups, the
+// parts kept in fp32 in the workspace and joined in a fixed order.
+#pragma once
+#include "common.h"
+
+namespace vaesne {
+namespace pk {
+
+typedef float f16v __attribute__((ext_vector_type(16)));
+typedef float f4 __attribute__((ext_vector_type(4)));
+typedef float f2 __attribute__((ext_vector_type(2)));
+typedef short s4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+typedef __bf16 b8 __attribute__((ext_vector_type(8)));
+typedef __bf16 b4 __attribute__((ext_vector_type(4)));
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef _Float16 h4 __attribute__((ext_vector_type(4)));
+
+template <class T> struct Ty;
+template <> struct Ty<float> { using Frag = f4; using Quad = f4; };
+template <> struct Ty<__bf16> { using Frag = b8; using Quad = b4; };
+template <> struct Ty<_Float16> { using Frag = h8; using Quad = h4; };
+
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr float INF = __builtin_inff();
+
+struct Args {
+  vaesne_packed_attn p;
+  int pg, nsub, group;         // heads per tile, tiles per key head's group, query heads per key head
+  uint32_t pgm;                // ceil(2^32 / pg), 0 for pg = 1
+  int nsplit;
+  float c;                     // scale * log2(e)
+  float* part;                 // split parts: [nsplit][rows][D] (dK / dV: dk parts, then dv parts)
+  float* part_lse;             // [nsplit][rows]
+  float* delta;                // [total_q][Hq]: rowsum(dO O)
+  float* hist;                 // [dQ workgroups][2R + 1]
+  uint32_t* domax;             // [Hkv]: bits of max |dO| (fp16)
+};
+
+__device__ __forceinline__ int div_pg(const Args& a, int row) {
+  return a.pgm ? (int)__umulhi((uint32_t)row, a.pgm) : row;
+}
+
+// ---- products ------------------------------------------------------------------------------
+__device__ __forceinline__ f16v mma(b8 a, b8 b, f16v c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f16v mma(h8 a, h8 b, f16v c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f16v mma(f4 a, f4 b, f16v c) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[j], b[j], c, 0, 0, 0);
+  return c;
+}
+
+// accumulator registers of contraction block t as the other operand's fragment.  16-bit types
+// round to nearest even here: P <= 2^8 and dS enter the matrix cores in the inputs' own type, the
+// sums stay fp32 (a relative 2^-9 (bf16) of each term, independent between terms)
+template <class T> __device__ __forceinline__ typename Ty<T>::Frag take(const f16v& s, int t) {
+  constexpr int N = 16 / sizeof(T);
+  float __attribute__((ext_vector_type(N))) v;
+#pragma unroll
+  for (int j = 0; j < N; ++j) v[j] = s[N * t + j];
+  return __builtin_convertvector(v, typename Ty<T>::Frag);
+}
+
+// ---- LDS tiles -----------------------------------------------------------------------------
+template <class T, int DP> struct Tile {
+  static constexpr int EPC = 16 / sizeof(T);          // elements per chunk
+  static constexpr int CPR = DP / EPC;                // chunks per row
+  static constexpr int RB = CPR * 16;                 // bytes per row
+  static constexpr int KC = 2 * EPC;                  // depth of one fragment product
+  static constexpr int NCH = DP / KC;                 // fragments per row
+  static constexpr int DT = (DP + 31) / 32;           // 32-column tiles
+  static constexpr int TB = 32 / KC;                  // contraction blocks per 32 rows
+
+  static __device__ __forceinline__ int swz(int r) {
+    if constexpr (CPR >= 16) return ((r & 3) << 2) | ((r >> 2) & 3);
+    else if constexpr (CPR == 8) return (((r >> 1) & 1) << 2) | ((r >> 2) & 3);
+    else if constexpr (CPR == 4) return (r >> 2) & 3;
+    else return (r >> 3) & 1;
+  }
+  static __device__ __forceinline__ int at(int r, int c) { return r * RB + ((c ^ swz(r)) << 4); }
+
+  // lane's fragment of row r: columns KC k + EPC h ..
+  static __device__ __forceinline__ typename Ty<T>::Frag row(const char* s, int r, int k, int h) {
+    return *reinterpret_cast<const typename Ty<T>::Frag*>(s + at(r, 2 * k + h));
+  }
+  // transposed fragment: column 32 dt + lane % 32 of rows r0 + (block t's slots)
+  static __device__ __forceinline__ typename Ty<T>::Frag col(const char* s, int r0, int t, int dt, int lane) {
+    const int h = lane >> 5;
+    if constexpr (sizeof(T) == 2) {
+      const int i = lane & 15, c = (4 * dt + 2 * ((lane >> 4) & 1) + ((i & 3) >> 1)) & (CPR - 1);
+      u4 o;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int r = r0 + KC * t + 8 * j + 4 * h + (i >> 2);
+        const s4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+            (__attribute__((address_space(3))) s4*)(s + at(r, c) + 8 * (i & 1)));
+        const uint2 y = __builtin_bit_cast(uint2, x);
+        o[2 * j] = y.x; o[2 * j + 1] = y.y;
+      }
+      return __builtin_bit_cast(typename Ty<T>::Frag, o);
+    } else {
+      const int d = 32 * dt + (lane & 31);
+      typename Ty<T>::Frag o;
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        o[j] = *reinterpret_cast<const float*>(s + at(r0 + KC * t + 4 * h + j, (d >> 2) & (CPR - 1)) + 4 * (d & 3));
+      return o;
+    }
+  }
+};
+
+// ROWS rows of a tile, global -> registers -> LDS (16-byte chunks; absent ones are zero)
+template <class T, int DP, int ROWS, int NT> struct Stage {
+  using L = Tile<T, DP>;
+  static constexpr int CH = ROWS * L::CPR;
+  static constexpr int NI = (CH + NT - 1) / NT;
+  u4 v[NI];
+  template <class RowPtr> __device__ __forceinline__ void load(int D, RowPtr row_ptr) {
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      const int id = threadIdx.x + i * NT, r = id / L::CPR, c = id % L::CPR;
+      v[i] = u4{0, 0, 0, 0};
+      if (CH % NT != 0 && id >= CH) continue;
+      const T* p = row_ptr(r);
+      if (p != nullptr && c * L::EPC < D) v[i] = *reinterpret_cast<const u4*>(p + c * L::EPC);
+    }
+  }
+  __device__ __forceinline__ void store(char* s) const {
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      const int id = threadIdx.x + i * NT;
+      if (CH % NT != 0 && id >= CH) continue;
+      *reinterpret_cast<u4*>(s + L::at(id / L::CPR, id % L::CPR)) = v[i];
+    }
+  }
+};
+
+template <class T, int DP> using Frags = typename Ty<T>::Frag[Tile<T, DP>::NCH];
+template <class T, int DP>
+__device__ __forceinline__ void load_frags(Frags<T, DP>& f, const T* p, int D, int h) {
+  using L = Tile<T, DP>;
+#pragma unroll
+  for (int k = 0; k < L::NCH; ++k) {
+    const int d = k * L::KC + h * L::EPC;
+    u4 x{0, 0, 0, 0};
+    if (p != nullptr && d < D) x = *reinterpret_cast<const u4*>(p + d);
+    f[k] = __builtin_bit_cast(typename Ty<T>::Frag, x);
+  }
+}
+
+// one column's accumulators (rows = features), scaled, to D consecutive elements
+template <class U, int DT>
+__device__ __forceinline__ void store_col(U* p, const f16v (&o)[DT], float f, int D, int h) {
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int d = 32 * dt + 8 * q + 4 * h;
+      if (d < D) {
+        const f4 x = {o[dt][4 * q] * f, o[dt][4 * q + 1] * f, o[dt][4 * q + 2] * f, o[dt][4 * q + 3] * f};
+        *reinterpret_cast<typename Ty<U>::Quad*>(p + d) = __builtin_convertvector(x, typename Ty<U>::Quad);
+      }
+    }
+}
+
+// the bias of every clamped relative position for one head, log2 domain
+template <class T, int NT>
+__device__ __forceinline__ void load_bias(const Args& a, float* lut, int head) {
+  const T* tb = reinterpret_cast<const T*>(a.p.table);
+  for (int i = threadIdx.x; i < 2 * a.p.max_distance + 1; i += NT) {
+    const int b = min(max(a.p.lut[i], 0), a.p.num_buckets - 1);
+    lut[i] = (float)tb[(int64_t)b * a.p.Hq + head] * LOG2E;
+  }
+}
+
+__device__ __forceinline__ int acc_row(int r, int h) { return 8 * (r >> 2) + 4 * h + (r & 3); }
+
+// where a workgroup's query tile lies
+struct QTile {
+  int seq, pos0, nq, nk, npos, nrows, off, kvh, head0;
+  int64_t q0, k0;
+  __device__ __forceinline__ QTile(const Args& a, int tile, int hidx) {
+    seq = a.p.q_tiles[2 * tile];
+    pos0 = a.p.q_tiles[2 * tile + 1];
+    q0 = a.p.cu_q[seq];
+    k0 = a.p.cu_k[seq];
+    nq = a.p.cu_q[seq + 1] - (int)q0;
+    nk = a.p.cu_k[seq + 1] - (int)k0;
+    off = nk - nq;
+    npos = min(a.p.q_tile, nq - pos0);
+    nrows = npos * a.pg;
+    kvh = hidx / a.nsub;
+    head0 = kvh * a.group + (hidx - kvh * a.nsub) * a.pg;
+  }
+  __device__ __forceinline__ int limit(const Args& a, int row) const {   // keys that row sees
+    return a.p.causal ? min(max(pos0 + div_pg(a, row) + off + 1, 0), nk) : nk;
+  }
+};
+
+// scores of one 32x32 tile to log2-domain values with bias: s c + bias
+template <int N>
+__device__ __forceinline__ void add_bias(f16v& s, float c, const float* lut, int rel0, int h, int R, int sign) {
+  // relative position of register r: rel0 + sign * acc_row(r, h)
+  (void)N;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) {
+    const int rel = rel0 + sign * acc_row(r, h);
+    s[r] = fmaf(s[r], c, lut[min(max(rel, -R), R) + R]);
+  }
+}
+
+// -------------------------------------------------------------------------------------------
+// forward
+// -------------------------------------------------------------------------------------------
+template <class T, int DP> constexpr int key_tile() { return sizeof(T) == 2 ? 64 : 32; }
+// waves per SIMD the registers are budgeted for: fp32 at head_dim 128 holds two operands of 64
+// registers beside 64 of sums, and takes the whole file
+template <class T, int DP> constexpr int occ() { return sizeof(T) == 4 && DP == 128 ? 1 : 2; }
+
+template <class T, int DP, bool BIAS, int NW>
+__global__ __launch_bounds__(NW * 64, (occ<T, DP>())) void fwd_kernel(Args a) {
+  using L = Tile<T, DP>;
+  constexpr int NT = NW * 64, BN = key_tile<T, DP>(), NB = BN / 32, TILE = BN * L::RB;
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  float* lut = reinterpret_cast<float*>(smem + 4 * TILE);
+  const int nh = a.p.Hkv * a.nsub;
+  const int hidx = blockIdx.x % nh;
+  const QTile t(a, blockIdx.x / nh, hidx);
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, h = lane >> 5, D = a.p.D, R = a.p.max_distance;
+  if (BIAS) load_bias<T, NT>(a, lut, t.head0);
+
+  const int row = w * 32 + (lane & 31), dpos = div_pg(a, row);
+  const bool valid = row < t.nrows;
+  const int head = t.head0 + row - dpos * a.pg;
+  const int lim = valid ? t.limit(a, row) : t.nk;
+  const int qabs = t.pos0 + dpos + t.off;
+  const bool active = w * 32 < t.nrows;
+  const int wmin = t.limit(a, w * 32), wmax = active ? t.limit(a, min(w * 32 + 31, t.nrows - 1)) : 0;
+  const int kend = t.limit(a, t.nrows - 1);
+  const int nt = (kend + BN - 1) / BN, per = (nt + a.nsplit - 1) / a.nsplit;
+  const int t0 = blockIdx.y * per, t1 = min(nt, t0 + per);
+
+  typename Ty<T>::Frag qf[L::NCH];
+  const T* qp = reinterpret_cast<const T*>(a.p.q) + (t.q0 + t.pos0 + dpos) * a.p.q_ts + (int64_t)head * a.p.q_hs;
+  load_frags<T, DP>(qf, valid ? qp : nullptr, D, h);
+
+  f16v o[L::DT];
+#pragma unroll
+  for (int i = 0; i < L::DT; ++i) o[i] = f16v{};
+  float m = -INF, l = 0.f;
+
+  const T* kb = reinterpret_cast<const T*>(a.p.k) + t.k0 * a.p.k_ts + t.kvh * a.p.k_hs;
+  const T* vb = reinterpret_cast<const T*>(a.p.v) + t.k0 * a.p.v_ts + t.kvh * a.p.v_hs;
+  Stage<T, DP, BN, NT> ks, vs;
+  auto fetch = [&](int j) {
+    ks.load(D, [&](int r) { const int key = j * BN + r; return key < t.nk ? kb + key * a.p.k_ts : nullptr; });
+    vs.load(D, [&](int r) { const int key = j * BN + r; return key < t.nk ? vb + key * a.p.v_ts : nullptr; });
+  };
+  if (t0 < t1) {
+    fetch(t0);
+    ks.store(smem);
+    vs.store(smem + TILE);
+  }
+  __syncthreads();
+  for (int j = t0; j < t1; ++j) {
+    const char* K = smem + ((j - t0) & 1) * 2 * TILE;
+    const char* V = K + TILE;
+    if (j + 1 < t1) fetch(j + 1);
+    const int base = j * BN;
+    if (base < wmax) {
+      f16v s[NB];
+#pragma unroll
+      for (int n = 0; n < NB; ++n) {
+        s[n] = f16v{};
+#pragma unroll
+        for (int k = 0; k < L::NCH; ++k) s[n] = mma(L::row(K, 32 * n + (lane & 31), k, h), qf[k], s[n]);
+      }
+      // scores to the units of the running maximum: raw without a bias, log2 with one
+      const float c = BIAS ? 1.f : a.c;
+      if (BIAS) {
+#pragma unroll
+        for (int n = 0; n < NB; ++n) add_bias<0>(s[n], a.c, lut, base + 32 * n - qabs, h, R, 1);
+      }
+      if (base + BN > wmin) {
+#pragma unroll
+        for (int n = 0; n < NB; ++n)
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            if (base + 32 * n + acc_row(r, h) >= lim) s[n][r] = -INF;
+      }
+      float mt = s[0][0];
+#pragma unroll
+      for (int n = 0; n < NB; ++n)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) mt = fmaxf(mt, s[n][r]);
+      mt = xmax32(mt);
+      // the origin moves only when a score exceeds it by 2^8: exp2 stays <= 2^8, sums fp32
+      if (__any(mt > m + 8.f / c)) {
+        const float mn = fmaxf(m, mt), f = mn == -INF ? 1.f : __builtin_amdgcn_exp2f((m - mn) * c);
+        m = mn;
+        l *= f;
+#pragma unroll
+        for (int i = 0; i < L::DT; ++i)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) o[i][r] *= f;
+      }
+      const float mc = m == -INF ? 0.f : -m * c;
+#pragma unroll
+      for (int n = 0; n < NB; ++n)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          s[n][r] = __builtin_amdgcn_exp2f(fmaf(s[n][r], c, mc));
+          l += s[n][r];
+        }
+#pragma unroll
+      for (int n = 0; n < NB; ++n)
+#pragma unroll
+        for (int b = 0; b < L::TB; ++b) {
+          const auto pf = take<T>(s[n], b);
+#pragma unroll
+          for (int dt = 0; dt < L::DT; ++dt) o[dt] = mma(L::col(V, 32 * n, b, dt, lane), pf, o[dt]);
+        }
+    }
+    if (j + 1 < t1) {
+      char* Kn = smem + ((j + 1 - t0) & 1) * 2 * TILE;
+      ks.store(Kn);
+      vs.store(Kn + TILE);
+    }
+    __syncthreads();
+  }
+  l = xsum32(l);
+  if (!valid) return;
+  const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);      // (a NaN sum stays one)
+  const float lse = l == 0.f ? INF : fmaf(m, BIAS ? 1.f : a.c, __log2f(l));
+  const int64_t rid = (t.q0 + t.pos0 + dpos) * a.p.Hq + head;
+  if (a.nsplit == 1) {
+    store_col(reinterpret_cast<T*>(a.p.o) + rid * D, o, inv, D, h);
+    if (h == 0) a.p.lse[rid] = lse;
+  } else {
+    const int64_t pid = (int64_t)blockIdx.y * a.p.total_q * a.p.Hq + rid;
+    store_col(a.part + pid * D, o, inv, D, h);
+    if (h == 0) a.part_lse[pid] = lse;
+  }
+}
+
+// Joins the parts of `rows` rows of D: weighted by their log-sum-exp (WEIGHTED: the forward; +inf
+// marks a part that saw nothing) or plainly summed, in the order of the parts.  8 rows per
+// workgroup, 32 lanes of 4 columns each.
+template <class T, bool WEIGHTED>
+__global__ __launch_bounds__(256) void join_kernel(const float* part, const float* part_lse, int n, int64_t rows,
+                                                   int D, T* out, float* lse) {
+  const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int d = (threadIdx.x & 31) * 4;
+  if (row >= rows) return;
+  f4 acc = {0.f, 0.f, 0.f, 0.f};
+  float m = -INF, sum = 0.f;
+  if (WEIGHTED) {
+    for (int i = 0; i < n; ++i) {
+      const float x = part_lse[i * rows + row];
+      if (x != INF) m = fmaxf(m, x);
+    }
+    for (int i = 0; i < n; ++i) {
+      const float x = part_lse[i * rows + row];
+      if (x != INF) sum += __builtin_amdgcn_exp2f(x - m);
+    }
+  }
+  if (d < D)
+    for (int i = 0; i < n; ++i) {
+      float wgt = 1.f;
+      if (WEIGHTED) {
+        const float x = part_lse[i * rows + row];
+        if (x == INF) continue;
+        wgt = __builtin_amdgcn_exp2f(x - m) / sum;
+      }
+      const f4 p = *reinterpret_cast<const f4*>(part + (i * rows + row) * D + d);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[e] = fmaf(wgt, p[e], acc[e]);
+    }
+  if (d < D) *reinterpret_cast<typename Ty<T>::Quad*>(out + row * D + d) = __builtin_convertvector(acc, typename Ty<T>::Quad);
+  if (WEIGHTED && d == 0) lse[row] = sum == 0.f ? INF : m + __log2f(sum);
+}
+
+// -------------------------------------------------------------------------------------------
+// backward: dQ (and rowsum(dO O), the bias sums by relative position)
+// -------------------------------------------------------------------------------------------
+// fp16 has few exponents: dS enters the products scaled by a power of two taken from |dO|, 2^-e with
+// max |dO| in [2^e, 2^(e+1)), times 2^-3 (|dP| < 2^-2 sum |v|); it is taken out of the fp32 results.
+// bf16 and fp32 have fp32's range and take 1.
+__device__ __forceinline__ float pow2_of(uint32_t bits) {   // 2^e of |x|, 1 for 0 / inf / NaN
+  const uint32_t e = bits >> 23;
+  return e == 0 || e >= 255 ? 1.f : __uint_as_float(e << 23);
+}
+
+template <class T, int DP, bool BIAS, int NW>
+__global__ __launch_bounds__(NW * 64, (occ<T, DP>())) void dq_kernel(Args a) {
+  using L = Tile<T, DP>;
+  constexpr int NT = NW * 64, BN = key_tile<T, DP>(), NB = BN / 32, TILE = BN * L::RB;
+  constexpr bool HALF = __is_same(T, _Float16);
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  const int R = a.p.max_distance, NH = 2 * R + 1;
+  float* lut = reinterpret_cast<float*>(smem + 4 * TILE);
+  float* hist = lut + NH + (threadIdx.x >> 6) * NH;            // this wave's sums by relative position
+  const int nh = a.p.Hkv * a.nsub;
+  const int hidx = blockIdx.x % nh;
+  const QTile t(a, blockIdx.x / nh, hidx);
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, h = lane >> 5, D = a.p.D;
+  const bool sums = BIAS && a.p.dtable != nullptr;
+  if (BIAS) load_bias<T, NT>(a, lut, t.head0);
+  if (sums)
+    for (int i = lane; i < NH; i += 64) hist[i] = 0.f;
+
+  const int row = w * 32 + (lane & 31), dpos = div_pg(a, row);
+  const bool valid = row < t.nrows;
+  const int head = t.head0 + row - dpos * a.pg;
+  const int lim = valid ? t.limit(a, row) : 0;
+  const int qabs = t.pos0 + dpos + t.off;
+  const bool active = w * 32 < t.nrows;
+  const int wmin = w * 32 + 31 < t.nrows ? t.limit(a, w * 32) : 0;
+  const int wmax = active ? t.limit(a, min(w * 32 + 31, t.nrows - 1)) : 0;
+  const int kend = t.limit(a, t.nrows - 1);
+  const int nt = (kend + BN - 1) / BN, per = (nt + a.nsplit - 1) / a.nsplit;
+  const int t0 = blockIdx.y * per, t1 = min(nt, t0 + per);
+
+  const int64_t tok = t.q0 + t.pos0 + dpos, rid = tok * a.p.Hq + head;
+  typename Ty<T>::Frag qf[L::NCH], gf[L::NCH];
+  load_frags<T, DP>(qf, valid ? reinterpret_cast<const T*>(a.p.q) + tok * a.p.q_ts + (int64_t)head * a.p.q_hs : nullptr, D, h);
+  load_frags<T, DP>(gf, valid ? reinterpret_cast<const T*>(a.p.dout) + tok * a.p.do_ts + (int64_t)head * a.p.do_hs : nullptr, D, h);
+  float delta = 0.f, big = 0.f;
+  {
+    typename Ty<T>::Frag of[L::NCH];
+    load_frags<T, DP>(of, valid ? reinterpret_cast<const T*>(a.p.o) + rid * D : nullptr, D, h);
+#pragma unroll
+    for (int k = 0; k < L::NCH; ++k)
+#pragma unroll
+      for (int e = 0; e < L::EPC; ++e) {
+        delta = fmaf((float)gf[k][e], (float)of[k][e], delta);
+        if (HALF) big = fmaxf(big, fabsf((float)gf[k][e]));
+      }
+  }
+  delta = xsum32(delta);
+  const float lse = valid ? a.p.lse[rid] : INF;
+  float up = 1.f;                                              // 1 / (the factor on dS)
+  if (HALF) {
+    big = xmax32(big);
+    up = 8.f * pow2_of(__float_as_uint(big));
+    if (blockIdx.y == 0) {                                     // for dK / dV: one factor per key head
+      const float wbig = wave_max(big);
+      if (lane == 0 && wbig > 0.f) atomicMax(a.domax + t.kvh, __float_as_uint(wbig));   // order-free
+    }
+  }
+  const float down = 1.f / up;
+  if (valid && h == 0 && blockIdx.y == 0) a.delta[rid] = delta;
+
+  f16v o[L::DT];
+#pragma unroll
+  for (int i = 0; i < L::DT; ++i) o[i] = f16v{};
+  float far_lo = 0.f, far_hi = 0.f;
+
+  const T* kb = reinterpret_cast<const T*>(a.p.k) + t.k0 * a.p.k_ts + t.kvh * a.p.k_hs;
+  const T* vb = reinterpret_cast<const T*>(a.p.v) + t.k0 * a.p.v_ts + t.kvh * a.p.v_hs;
+  Stage<T, DP, BN, NT> ks, vs;
+  auto fetch = [&](int j) {
+    ks.load(D, [&](int r) { const int key = j * BN + r; return key < t.nk ? kb + key * a.p.k_ts : nullptr; });
+    vs.load(D, [&](int r) { const int key = j * BN + r; return key < t.nk ? vb + key * a.p.v_ts : nullptr; });
+  };
+  if (t0 < t1) {
+    fetch(t0);
+    ks.store(smem);
+    vs.store(smem + TILE);
+  }
+  __syncthreads();
+  for (int j = t0; j < t1; ++j) {
+    const char* K = smem + ((j - t0) & 1) * 2 * TILE;
+    const char* V = K + TILE;
+    if (j + 1 < t1) fetch(j + 1);
+#pragma unroll
+    for (int n = 0; n < NB; ++n) {
+      const int base = j * BN + 32 * n;
+      if (base < wmax) {
+        f16v s = f16v{}, g = f16v{};
+#pragma unroll
+        for (int k = 0; k < L::NCH; ++k) s = mma(L::row(K, 32 * n + (lane & 31), k, h), qf[k], s);
+#pragma unroll
+        for (int k = 0; k < L::NCH; ++k) g = mma(L::row(V, 32 * n + (lane & 31), k, h), gf[k], g);
+        const float c = BIAS ? 1.f : a.c;
+        const int rel0 = base - qabs;
+        if (BIAS) add_bias<0>(s, a.c, lut, rel0, h, R, 1);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c, -lse)) * (g[r] - delta);
+        if (base + 32 > wmin) {
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            if (base + acc_row(r, h) >= lim) s[r] = 0.f;
+        }
+        if (sums) {
+          // wave-uniform: the tile lies beyond +-R for every row (row 0's and row 31's distances)
+          const int lo = base - (t.pos0 + w * 32 + 31 + t.off), hi = base + 31 - (t.pos0 + w * 32 + t.off);
+          if (hi <= -R) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) far_lo += s[r];
+          } else if (lo >= R) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) far_hi += s[r];
+          } else {
+            // one half of the wave at a time: the 32 lanes of a half meet 32 different distances in
+            // each register and a wave's LDS operations keep their order, so every sum of this
+            // wave-private array is taken in one fixed order
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+              const int rel = rel0 + acc_row(r, h);
+              if (rel <= -R) far_lo += s[r];
+              else if (rel >= R) far_hi += s[r];
+            }
+            for (int half = 0; half < 2; ++half) {
+              if (h == half) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                  const int rel = rel0 + acc_row(r, h);
+                  if (rel > -R && rel < R)
+                    __hip_atomic_fetch_add(hist + rel + R, s[r], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WAVEFRONT);
+                }
+              }
+            }
+          }
+        }
+        if (HALF) {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) s[r] *= down;
+        }
+#pragma unroll
+        for (int b = 0; b < L::TB; ++b) {
+          const auto sf = take<T>(s, b);
+#pragma unroll
+          for (int dt = 0; dt < L::DT; ++dt) o[dt] = mma(L::col(K, 32 * n, b, dt, lane), sf, o[dt]);
+        }
+      }
+    }
+    if (j + 1 < t1) {
+      char* Kn = smem + ((j + 1 - t0) & 1) * 2 * TILE;
+      ks.store(Kn);
+      vs.store(Kn + TILE);
+    }
+    __syncthreads();
+  }
+  if (sums) {
+    far_lo = wave_sum(far_lo);
+    far_hi = wave_sum(far_hi);
+    if (lane == 0) {
+      hist[0] = far_lo;
+      hist[2 * R] += far_hi;                                   // R >= 1: its own slot
+    }
+    __syncthreads();
+    float* out = a.hist + ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * NH;
+    for (int i = threadIdx.x; i < NH; i += NT) {
+      float x = 0.f;
+#pragma unroll
+      for (int v = 0; v < NW; ++v) x += lut[NH + v * NH + i];
+      out[i] = x;
+    }
+  }
+  if (!valid) return;
+  const float f = a.p.scale * up;
+  if (a.nsplit == 1) store_col(reinterpret_cast<T*>(a.p.dq) + rid * D, o, f, D, h);
+  else store_col(a.part + ((int64_t)blockIdx.y * a.p.total_q * a.p.Hq + rid) * D, o, f, D, h);
+}
+
+// sums by relative position of the n workgroups of a head (workgroup i * Hq + head), 16 slices of
+// them in order, then the slices in order: rel[head][NH]
+__global__ __launch_bounds__(1024) void hist_sum_kernel(const float* hist, int n, int Hq, int NH, float* rel);
+// dtable[b][head] = sum of rel[head][i] over the relative positions i of bucket b, in order
+template <class T>
+__global__ __launch_bounds__(256) void hist_bucket_kernel(const float* rel, const int32_t* lut, int NH, int Hq, int nb,
+                                                          T* dtable) {
+  extern __shared__ float sm[];
+  int* bucket = reinterpret_cast<int*>(sm + NH);
+  for (int i = threadIdx.x; i < NH; i += 256) {
+    sm[i] = rel[(int64_t)blockIdx.x * NH + i];
+    bucket[i] = min(max(lut[i], 0), nb - 1);
+  }
+  __syncthreads();
+  for (int b = threadIdx.x; b < nb; b += 256) {
+    float x = 0.f;
+    for (int i = 0; i < NH; ++i) x += bucket[i] == b ? sm[i] : 0.f;
+    dtable[(int64_t)b * Hq + blockIdx.x] = (T)x;
+  }
+}
+
+// -------------------------------------------------------------------------------------------
+// backward: dK, dV
+// -------------------------------------------------------------------------------------------
+template <class T, int DP, bool BIAS, int NW>
+__global__ __launch_bounds__(NW * 64, (occ<T, DP>())) void dkv_kernel(Args a) {
+  using L = Tile<T, DP>;
+  constexpr int NT = NW * 64, BQ = key_tile<T, DP>(), NB = BQ / 32, TILE = BQ * L::RB;
+  constexpr bool HALF = __is_same(T, _Float16);
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  float* stat = reinterpret_cast<float*>(smem + 4 * TILE);     // [2][lse BQ | delta BQ]
+  float* lut = stat + 4 * BQ;
+  const int kvh = blockIdx.x % a.p.Hkv, tile = blockIdx.x / a.p.Hkv, D = a.p.D, R = a.p.max_distance;
+  const int seq = a.p.k_tiles[2 * tile], key0 = a.p.k_tiles[2 * tile + 1];
+  const int64_t q0 = a.p.cu_q[seq], k0 = a.p.cu_k[seq];
+  const int nq = a.p.cu_q[seq + 1] - (int)q0, nk = a.p.cu_k[seq + 1] - (int)k0, off = nk - nq;
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, h = lane >> 5;
+  const int key = key0 + w * 32 + (lane & 31);
+  const bool valid = key < nk;
+  typename Ty<T>::Frag kf[L::NCH], vf[L::NCH];
+  load_frags<T, DP>(kf, valid ? reinterpret_cast<const T*>(a.p.k) + (k0 + key) * a.p.k_ts + kvh * a.p.k_hs : nullptr, D, h);
+  load_frags<T, DP>(vf, valid ? reinterpret_cast<const T*>(a.p.v) + (k0 + key) * a.p.v_ts + kvh * a.p.v_hs : nullptr, D, h);
+  f16v dk[L::DT], dv[L::DT];
+#pragma unroll
+  for (int i = 0; i < L::DT; ++i) dk[i] = dv[i] = f16v{};
+  float up = 1.f;
+  if (HALF) up = 8.f * pow2_of(a.domax[kvh]);
+  const float down = 1.f / up;
+
+  // rows (position * PG + head) that see any of the tile's keys, tile by tile, one head group after
+  // the other: it = sub * ntq + row tile
+  const int nrows = nq * a.pg;
+  const int first = a.p.causal ? min(max(key0 - off, 0), nq) * a.pg / BQ : 0;
+  const int ntq = max((nrows + BQ - 1) / BQ - first, 0), total = a.nsub * ntq;
+  const int per = (total + a.nsplit - 1) / a.nsplit, t0 = blockIdx.y * per, t1 = min(total, t0 + per);
+  // the first row that sees this lane's key / the wave's first and last key
+  const int see = a.p.causal ? (key - off) * a.pg : 0;
+  const int wfirst = a.p.causal ? (key0 + w * 32 - off) * a.pg : 0;
+  const int wlast = a.p.causal ? (key0 + w * 32 + 31 - off) * a.pg : 0;
+  const bool active = key0 + w * 32 < nk;
+
+  Stage<T, DP, BQ, NT> qs, gs;
+  float st_l = INF, st_d = 0.f;
+  auto fetch = [&](int it) {
+    const int sub = it / ntq, rb = (first + it - sub * ntq) * BQ;
+    const int head0 = kvh * a.group + sub * a.pg;
+    auto ptr = [&](const void* x, int64_t ts, int64_t hs, int r) -> const T* {
+      const int rr = rb + r;
+      if (rr >= nrows) return nullptr;
+      const int pos = div_pg(a, rr);
+      return reinterpret_cast<const T*>(x) + (q0 + pos) * ts + (int64_t)(head0 + rr - pos * a.pg) * hs;
+    };
+    qs.load(D, [&](int r) { return ptr(a.p.q, a.p.q_ts, a.p.q_hs, r); });
+    gs.load(D, [&](int r) { return ptr(a.p.dout, a.p.do_ts, a.p.do_hs, r); });
+    if (threadIdx.x < BQ) {
+      const int rr = rb + threadIdx.x;
+      st_l = INF;
+      st_d = 0.f;
+      if (rr < nrows) {
+        const int pos = div_pg(a, rr);
+        const int64_t rid = (q0 + pos) * a.p.Hq + head0 + rr - pos * a.pg;
+        st_l = a.p.lse[rid];
+        st_d = a.delta[rid];
+      }
+    }
+  };
+  auto commit = [&](int b) {
+    qs.store(smem + b * 2 * TILE);
+    gs.store(smem + b * 2 * TILE + TILE);
+    if (threadIdx.x < BQ) {
+      stat[b * 2 * BQ + threadIdx.x] = st_l;
+      stat[b * 2 * BQ + BQ + threadIdx.x] = st_d;
+    }
+  };
+  int sub_now = -1;
+  if (t0 < t1) {
+    fetch(t0);
+    commit(0);
+  }
+  __syncthreads();
+  for (int it = t0; it < t1; ++it) {
+    const int b = (it - t0) & 1;
+    const char* Q = smem + b * 2 * TILE;
+    const char* G = Q + TILE;
+    const float* lse = stat + b * 2 * BQ;
+    const float* dl = lse + BQ;
+    const int sub = it / ntq, rb = (first + it - sub * ntq) * BQ;
+    if (BIAS && sub != sub_now) {                              // the next head's biases
+      __syncthreads();
+      load_bias<T, NT>(a, lut, kvh * a.group + sub * a.pg);
+      __syncthreads();
+      sub_now = sub;
+    }
+    if (it + 1 < t1) fetch(it + 1);
+#pragma unroll
+    for (int n = 0; n < NB; ++n) {
+      const int base = rb + 32 * n;
+      if (active && base < nrows && base + 31 >= wfirst) {
+        f16v s = f16v{}, g = f16v{};
+#pragma unroll
+        for (int k = 0; k < L::NCH; ++k) s = mma(L::row(Q, 32 * n + (lane & 31), k, h), kf[k], s);
+        if (BIAS) add_bias<0>(s, a.c, lut, key - off - base, h, R, -1);
+        const float c = BIAS ? 1.f : a.c;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const f4 x = *reinterpret_cast<const f4*>(lse + 32 * n + 8 * q + 4 * h);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[4 * q + e] = __builtin_amdgcn_exp2f(fmaf(s[4 * q + e], c, -x[e]));
+        }
+        if (base < wlast) {
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            if (base + acc_row(r, h) < see) s[r] = 0.f;
+        }
+#pragma unroll
+        for (int t = 0; t < L::TB; ++t) {
+          const auto pf = take<T>(s, t);
+#pragma unroll
+          for (int dt = 0; dt < L::DT; ++dt) dv[dt] = mma(L::col(G, 32 * n, t, dt, lane), pf, dv[dt]);
+        }
+#pragma unroll
+        for (int k = 0; k < L::NCH; ++k) g = mma(L::row(G, 32 * n + (lane & 31), k, h), vf[k], g);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const f4 x = *reinterpret_cast<const f4*>(dl + 32 * n + 8 * q + 4 * h);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[4 * q + e] *= (g[4 * q + e] - x[e]) * (HALF ? down : 1.f);
+        }
+#pragma unroll
+        for (int t = 0; t < L::TB; ++t) {
+          const auto sf = take<T>(s, t);
+#pragma unroll
+          for (int dt = 0; dt < L::DT; ++dt) dk[dt] = mma(L::col(Q, 32 * n, t, dt, lane), sf, dk[dt]);
+        }
+      }
+    }
+    if (it + 1 < t1) commit(1 - b);
+    __syncthreads();
+  }
+  if (!valid) return;
+  const int64_t rid = (k0 + key) * a.p.Hkv + kvh, rows = a.p.total_k * a.p.Hkv;
+  if (a.nsplit == 1) {
+    store_col(reinterpret_cast<T*>(a.p.dk) + rid * D, dk, a.p.scale * up, D, h);
+    store_col(reinterpret_cast<T*>(a.p.dv) + rid * D, dv, 1.f, D, h);
+  } else {
+    store_col(a.part + ((int64_t)blockIdx.y * rows + rid) * D, dk, a.p.scale * up, D, h);
+    store_col(a.part + ((int64_t)(a.nsplit + blockIdx.y) * rows + rid) * D, dv, 1.f, D, h);
+  }
+}
+
+// ---- host: one launcher per type (packed_attention_<type>.hip) ------------------------------
+struct Plan {
+  Args a;
+  int dp, nwq, nwk, split_q, split_k;
+  int64_t part_bytes, delta_bytes, hist_bytes, rel_bytes, dom_bytes;   // carved in this order
+};
+template <class T> int run_fwd(const Plan& p, hipStream_t s);
+template <class T> int run_bwd(const Plan& p, hipStream_t s);
+
+template <class T, class K> int launch(K kernel, dim3 grid, int threads, size_t lds, const Args& a, hipStream_t s) {
+  if (lds > 65536) {
+    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
+                                             hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
+    if (e != hipSuccess) return (int)e;
+  }
+  hipLaunchKernelGGL(kernel, grid, dim3(threads), lds, s, a);
+  VAESNE_CHECK_LAUNCH();
+  return 0;
+}
+
+template <class T, int DP, bool BIAS> int fwd_dp(const Plan& p, hipStream_t s) {
+  Args a = p.a;
+  a.nsplit = p.split_q;
+  const int wgs = a.p.n_q_tiles * a.p.Hkv * a.nsub;
+  const size_t lds = 4 * key_tile<T, DP>() * Tile<T, DP>::RB + (BIAS ? (2 * a.p.max_distance + 1) * 4 : 0);
+  const int rc = p.nwq == 2 ? launch<T>(fwd_kernel<T, DP, BIAS, 2>, dim3(wgs, a.nsplit), 128, lds, a, s)
+                            : launch<T>(fwd_kernel<T, DP, BIAS, 4>, dim3(wgs, a.nsplit), 256, lds, a, s);
+  if (rc || a.nsplit == 1) return rc;
+  const int64_t rows = a.p.total_q * a.p.Hq;
+  hipLaunchKernelGGL((join_kernel<T, true>), dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, s, a.part, a.part_lse, a.nsplit,
+                     rows, a.p.D, reinterpret_cast<T*>(a.p.o), a.p.lse);
+  VAESNE_CHECK_LAUNCH();
+  return 0;
+}
+
+__global__ __launch_bounds__(64) void clear_kernel(uint32_t* p, int n);
+
+template <class T, int DP, bool BIAS> int bwd_dp(const Plan& p, hipStream_t s) {
+  Args a = p.a;
+  const int NH = 2 * a.p.max_distance + 1;
+  constexpr int BN = key_tile<T, DP>(), RB = Tile<T, DP>::RB;
+  if (__is_same(T, _Float16)) {
+    hipLaunchKernelGGL(clear_kernel, dim3((a.p.Hkv + 63) / 64), dim3(64), 0, s, a.domax, a.p.Hkv);
+    VAESNE_CHECK_LAUNCH();
+  }
+  if (a.p.n_q_tiles > 0) {
+    a.nsplit = p.split_q;
+    const int wgs = a.p.n_q_tiles * a.p.Hkv * a.nsub;
+    const size_t lds = 4 * BN * RB + (BIAS ? (1 + p.nwq) * NH * 4 : 0);
+    const int rc = p.nwq == 2 ? launch<T>(dq_kernel<T, DP, BIAS, 2>, dim3(wgs, a.nsplit), 128, lds, a, s)
+                              : launch<T>(dq_kernel<T, DP, BIAS, 4>, dim3(wgs, a.nsplit), 256, lds, a, s);
+    if (rc) return rc;
+    if (a.nsplit > 1) {
+      const int64_t rows = a.p.total_q * a.p.Hq;
+      hipLaunchKernelGGL((join_kernel<T, false>), dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, s, a.part, nullptr,
+                         a.nsplit, rows, a.p.D, reinterpret_cast<T*>(a.p.dq), nullptr);
+      VAESNE_CHECK_LAUNCH();
+    }
+  }
+  if (BIAS && a.p.dtable) {
+    float* rel = a.hist + p.hist_bytes / 4;
+    hipLaunchKernelGGL(hist_sum_kernel, dim3((NH + 63) / 64, a.p.Hq), dim3(1024), 0, s, a.hist,
+                       a.p.n_q_tiles * p.split_q, a.p.Hq, NH, rel);
+    VAESNE_CHECK_LAUNCH();
+    hipLaunchKernelGGL((hist_bucket_kernel<T>), dim3(a.p.Hq), dim3(256), NH * 8, s, rel, a.p.lut, NH, a.p.Hq,
+                       a.p.num_buckets, reinterpret_cast<T*>(a.p.dtable));
+    VAESNE_CHECK_LAUNCH();
+  }
+  if (a.p.n_k_tiles == 0) return 0;
+  a.nsplit = p.split_k;
+  const size_t lds = 4 * BN * RB + 16 * BN + (BIAS ? NH * 4 : 0);
+  const int wgs = a.p.n_k_tiles * a.p.Hkv;
+  const int rc = p.nwk == 2 ? launch<T>(dkv_kernel<T, DP, BIAS, 2>, dim3(wgs, a.nsplit), 128, lds, a, s)
+                            : launch<T>(dkv_kernel<T, DP, BIAS, 4>, dim3(wgs, a.nsplit), 256, lds, a, s);
+  if (rc || a.nsplit == 1) return rc;
+  const int64_t rows = a.p.total_k * a.p.Hkv;
+  for (int i = 0; i < 2; ++i) {
+    hipLaunchKernelGGL((join_kernel<T, false>), dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, s,
+                       a.part + (int64_t)i * a.nsplit * rows * a.p.D, nullptr, a.nsplit, rows, a.p.D,
+                       reinterpret_cast<T*>(i ? a.p.dv : a.p.dk), nullptr);
+    VAESNE_CHECK_LAUNCH();
+  }
+  return 0;
+}
+
+template <class T, bool BWD> int dispatch(const Plan& p, hipStream_t s) {
+#define VAESNE_PK(DPV)                                                                          \
+  if (p.dp == DPV) {                                                                            \
+    if constexpr (BWD) return p.a.p.table ? bwd_dp<T, DPV, true>(p, s) : bwd_dp<T, DPV, false>(p, s); \
+    else return p.a.p.table ? fwd_dp<T, DPV, true>(p, s) : fwd_dp<T, DPV, false>(p, s);         \
+  }
+  VAESNE_PK(16) VAESNE_PK(32) VAESNE_PK(64) VAESNE_PK(128)
+#undef VAESNE_PK
+  return (int)hipErrorInvalidValue;
+}
+
+}  // namespace pk
+}  // namespace vaesne

@@ -1,0 +1,191 @@
+// Packed-sequence attention: argument checks, the choice of tiles and splits, the small kernels
+// (packed_attention.h has the attention kernels, packed_attention_<type>.hip their instances).
+#include <algorithm>
+
+#include "packed_attention.h"
+
+using namespace vaesne;
+using namespace vaesne::pk;
+
+namespace vaesne {
+namespace pk {
+
+template <> int run_fwd<float>(const Plan& p, hipStream_t s);
+template <> int run_fwd<__bf16>(const Plan& p, hipStream_t s);
+template <> int run_fwd<_Float16>(const Plan& p, hipStream_t s);
+template <> int run_bwd<float>(const Plan& p, hipStream_t s);
+template <> int run_bwd<__bf16>(const Plan& p, hipStream_t s);
+template <> int run_bwd<_Float16>(const Plan& p, hipStream_t s);
+
+__global__ __launch_bounds__(64) void clear_kernel(uint32_t* p, int n) {
+  const int i = blockIdx.x * 64 + threadIdx.x;
+  if (i < n) p[i] = 0;
+}
+
+__global__ __launch_bounds__(1024) void hist_sum_kernel(const float* hist, int n, int Hq, int NH, float* rel) {
+  __shared__ float part[16][64];
+  const int c = blockIdx.x * 64 + (threadIdx.x & 63), slice = threadIdx.x >> 6, head = blockIdx.y;
+  float x = 0.f;
+  if (c < NH)
+    for (int i = slice; i < n; i += 16) x += hist[((int64_t)i * Hq + head) * NH + c];
+  part[slice][threadIdx.x & 63] = x;
+  __syncthreads();
+  if (slice == 0 && c < NH) {
+    x = 0.f;
+    for (int i = 0; i < 16; ++i) x += part[i][threadIdx.x];
+    rel[(int64_t)head * NH + c] = x;
+  }
+}
+
+namespace {
+
+constexpr int SLOTS = 512;            // workgroups the chip runs at once: two of 64 KB LDS per CU
+constexpr int MAX_SPLIT = 64;
+constexpr int64_t MAX_PART = 256 << 20;
+constexpr int64_t MAX_ROWS = 1 << 25; // rows of one sequence: 32-bit row arithmetic with room
+
+// Parts to cut the streamed axis into.  Each of `wgs` workgroups walks up to `longest` tiles, `mean` on
+// average.  A part shorter than 4 tiles costs more in joining than it saves; one longer than twice
+// the chip's mean share leaves the other CUs idle at the end.
+int splits(int64_t wgs, int64_t longest, double mean, int64_t part_bytes) {
+  const double share = std::max(4.0, wgs * mean / SLOTS);
+  if (longest < 1.5 * share) return 1;
+  int64_t n = (int64_t)((longest + share - 1) / share);
+  n = std::min<int64_t>(n, MAX_SPLIT);
+  n = std::min<int64_t>(n, std::max<int64_t>(1, MAX_PART / std::max<int64_t>(part_bytes, 1)));
+  return (int)std::max<int64_t>(n, 1);
+}
+
+int64_t up16(int64_t n) { return (n + 15) & ~(int64_t)15; }
+
+bool sizes_ok(const vaesne_packed_attn* a) {
+  return a && a->type >= 0 && a->type <= 2 && a->Hq > 0 && a->Hkv > 0 && a->Hq % a->Hkv == 0 && a->D > 0 &&
+         a->D <= 128 && a->D % 8 == 0 && a->nseq >= 0 && a->max_q >= 0 && a->max_k >= 0 && a->total_q >= 0 &&
+         a->total_k >= 0 && a->scale > 0.f && a->Hq <= 4096 &&
+         (a->table == nullptr || (a->max_distance >= 1 && a->max_distance <= 512 && a->num_buckets >= 1));
+}
+
+// query heads of a key head that share a tile: the largest divisor of the group that a 64-row tile
+// holds; one with a bias, whose table differs from head to head
+int heads_per_tile(const vaesne_packed_attn* a) {
+  if (a->table) return 1;
+  const int g = a->Hq / a->Hkv;
+  for (int p = std::min(g, 32); p > 1; --p)
+    if (g % p == 0) return p;
+  return 1;
+}
+
+int waves_for(int64_t rows) { return rows <= 64 ? 2 : 4; }
+
+int make_plan(const vaesne_packed_attn* a, Plan* p) {
+  if (!sizes_ok(a)) return (int)hipErrorInvalidValue;
+  *p = Plan{};
+  p->a.p = *a;
+  p->a.group = a->Hq / a->Hkv;
+  p->a.pg = heads_per_tile(a);
+  p->a.nsub = p->a.group / p->a.pg;
+  p->a.pgm = p->a.pg == 1 ? 0u : (uint32_t)(((1ull << 32) + p->a.pg - 1) / p->a.pg);
+  if ((int64_t)a->max_q * p->a.pg > MAX_ROWS || (int64_t)a->max_k * p->a.pg > MAX_ROWS) return (int)hipErrorInvalidValue;
+  p->a.c = a->scale * LOG2E;
+  p->dp = a->D <= 16 ? 16 : a->D <= 32 ? 32 : a->D <= 64 ? 64 : 128;
+  p->nwq = waves_for((int64_t)a->max_q * p->a.pg);
+  p->nwk = waves_for(a->max_k);
+  const int bn = a->type == 0 ? 32 : 64;
+  const int64_t qrows = a->total_q * a->Hq, krows = a->total_k * a->Hkv;
+  const double n = std::max(a->nseq, 1);
+  p->split_q = splits((int64_t)a->n_q_tiles * a->Hkv * p->a.nsub, (a->max_k + bn - 1) / bn, a->total_k / n / bn,
+                      qrows * (a->D + 1) * 4);
+  p->split_k = splits((int64_t)a->n_k_tiles * a->Hkv, (int64_t)p->a.nsub * (((int64_t)a->max_q * p->a.pg + bn - 1) / bn),
+                      (double)p->a.group * a->total_q / n / bn, 2 * krows * a->D * 4);
+  return 0;
+}
+
+// the workspace: split parts, their statistics | rowsum(dO O) | bias sums | max |dO|
+int64_t carve(Plan* p, int backward) {
+  const vaesne_packed_attn& a = p->a.p;
+  const int64_t qrows = a.total_q * a.Hq, krows = a.total_k * a.Hkv, NH = 2 * a.max_distance + 1;
+  int64_t part = 0;
+  if (p->split_q > 1) part = p->split_q * qrows * a.D * 4;
+  if (backward && p->split_k > 1) part = std::max(part, 2 * p->split_k * krows * a.D * 4);
+  p->part_bytes = up16(part);
+  const int64_t lse = !backward && p->split_q > 1 ? up16(p->split_q * qrows * 4) : 0;
+  p->delta_bytes = backward ? up16(qrows * 4) : 0;
+  const bool bias = backward && a.table && a.dtable;
+  p->hist_bytes = bias ? up16((int64_t)a.n_q_tiles * a.Hq * p->split_q * NH * 4) : 0;
+  p->rel_bytes = bias ? up16((int64_t)a.Hq * NH * 4) : 0;
+  p->dom_bytes = backward && a.type == 2 ? up16((int64_t)a.Hkv * 4) : 0;
+  char* w = reinterpret_cast<char*>(a.workspace);
+  p->a.part = reinterpret_cast<float*>(w);
+  p->a.part_lse = reinterpret_cast<float*>(w + p->part_bytes);
+  w += p->part_bytes + lse;
+  p->a.delta = reinterpret_cast<float*>(w);
+  p->a.hist = reinterpret_cast<float*>(w + p->delta_bytes);
+  p->a.domax = reinterpret_cast<uint32_t*>(w + p->delta_bytes + p->hist_bytes + p->rel_bytes);
+  return p->part_bytes + lse + p->delta_bytes + p->hist_bytes + p->rel_bytes + p->dom_bytes;
+}
+
+bool aligned(const void* p, int64_t ts, int64_t hs, int size) {
+  return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && (ts * size) % 16 == 0 && (hs * size) % 16 == 0;
+}
+
+int check(const Plan& p, int64_t bytes, int backward) {
+  const vaesne_packed_attn& a = p.a.p;
+  const int size = a.type == 0 ? 4 : 2;
+  const int bad = (int)hipErrorInvalidValue;
+  if (!a.cu_q || !a.cu_k) return bad;
+  if (a.q_tile != p.nwq * 32 / p.a.pg || a.k_tile != p.nwk * 32) return bad;
+  if (a.n_q_tiles < 0 || a.n_k_tiles < 0 || (a.total_q > 0 && (a.n_q_tiles == 0 || !a.q_tiles || !a.q || !a.o || !a.lse)) ||
+      (a.total_k > 0 && (!a.k || !a.v)))
+    return bad;
+  if (!aligned(a.q, a.q_ts, a.q_hs, size) || !aligned(a.k, a.k_ts, a.k_hs, size) || !aligned(a.v, a.v_ts, a.v_hs, size) ||
+      !aligned(a.o, 0, 0, size))
+    return bad;
+  if (a.table && !a.lut) return bad;
+  if (bytes > 0 && (!a.workspace || (reinterpret_cast<uintptr_t>(a.workspace) & 15))) return bad;
+  if ((int64_t)a.n_q_tiles * a.Hq >= (1ll << 31) || (int64_t)a.n_k_tiles * a.Hkv >= (1ll << 31)) return bad;
+  if (backward) {
+    if (a.total_q > 0 && (!a.dout || !a.dq)) return bad;
+    if (a.total_k > 0 && (!a.dk || !a.dv || a.n_k_tiles == 0 || !a.k_tiles)) return bad;
+    if (!aligned(a.dout, a.do_ts, a.do_hs, size) || !aligned(a.dq, 0, 0, size) || !aligned(a.dk, 0, 0, size) ||
+        !aligned(a.dv, 0, 0, size))
+      return bad;
+  }
+  return 0;
+}
+
+}  // namespace
+}  // namespace pk
+}  // namespace vaesne
+
+VAESNE_API int vaesne_packed_attn_tiles(const vaesne_packed_attn* a, int* q_tile, int* k_tile) {
+  Plan p;
+  const int rc = make_plan(a, &p);
+  if (rc) return rc;
+  *q_tile = p.nwq * 32 / p.a.pg;
+  *k_tile = p.nwk * 32;
+  return 0;
+}
+
+VAESNE_API int64_t vaesne_packed_attn_workspace(const vaesne_packed_attn* a, int backward) {
+  Plan p;
+  if (make_plan(a, &p)) return -1;
+  return carve(&p, backward);
+}
+
+VAESNE_API int vaesne_packed_attn_fwd(const vaesne_packed_attn* a, void* stream) {
+  Plan p;
+  int rc = make_plan(a, &p);
+  if (!rc) rc = check(p, carve(&p, 0), 0);
+  if (rc || a->total_q == 0) return rc;
+  hipStream_t s = (hipStream_t)stream;
+  return a->type == 0 ? run_fwd<float>(p, s) : a->type == 1 ? run_fwd<__bf16>(p, s) : run_fwd<_Float16>(p, s);
+}
+
+VAESNE_API int vaesne_packed_attn_bwd(const vaesne_packed_attn* a, void* stream) {
+  Plan p;
+  int rc = make_plan(a, &p);
+  if (!rc) rc = check(p, carve(&p, 1), 1);
+  if (rc) return rc;
+  hipStream_t s = (hipStream_t)stream;
+  return a->type == 0 ? run_bwd<float>(p, s) : a->type == 1 ? run_bwd<__bf16>(p, s) : run_bwd<_Float16>(p, s);
+}
