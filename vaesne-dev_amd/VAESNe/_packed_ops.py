@@ -279,7 +279,7 @@ def _head_rows(t):
     """t [T, H, D] with unit-stride, 16-byte aligned rows (a copy where it has none)."""
     n = t.element_size()
     s = t.stride()
-    if s[2] == 1 and s[0] * n % 16 == 0 and s[1] * n % 16 == 0 and t.data_ptr() % 16 == 0:
+    if s[2] == 1 and s[0] * n % 16 == 0 and s[1] * n % 16 == 0 and t.data_ptr() % 16 == 0 and max(s) < 1 << 22:
         return t
     return t.clone(memory_format=torch.contiguous_format)
 

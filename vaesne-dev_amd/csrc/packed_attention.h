@@ -99,6 +99,7 @@ template <class T, int DP> struct Tile {
   static constexpr int NCH = DP / KC;                 // fragments per row
   static constexpr int DT = (DP + 31) / 32;           // 32-column tiles
   static constexpr int TB = 32 / KC;                  // contraction blocks per 32 rows
+  static constexpr int CR = sizeof(T) == 2 ? 2 : 4;   // LDS reads of a transposed fragment
 
   static __device__ __forceinline__ int swz(int r) {
     if constexpr (CPR >= 16) return ((r & 3) << 2) | ((r >> 2) & 3);
@@ -138,21 +139,38 @@ template <class T, int DP> struct Tile {
   }
 };
 
-// ROWS rows of a tile, global -> registers -> LDS (16-byte chunks; absent ones are zero)
-template <class T, int DP, int ROWS, int NT> struct Stage {
+// ROWS rows of a tile, global -> registers -> LDS (16-byte chunks; absent ones are zero).  A thread's
+// offsets from the tile's first row never change, so a tile costs one buffer descriptor (scalar) and
+// no address arithmetic; an absent chunk's offset lies outside the descriptor and reads as zero.
+// (With 64-bit addresses computed for every chunk the forward issued 10 vector instructions per
+// score, with this 6.)  EVEN: rows lie at one stride, and a thread's chunks differ by a scalar step.
+constexpr uint32_t NO_ROW = 0x80000000u;
+template <class T, int DP, int ROWS, int NT, bool EVEN> struct Stage {
   using L = Tile<T, DP>;
   static constexpr int CH = ROWS * L::CPR;
   static constexpr int NI = (CH + NT - 1) / NT;
+  static constexpr int RS = NT / L::CPR;              // rows between a thread's chunks
   u4 v[NI];
-  template <class RowPtr> __device__ __forceinline__ void load(int D, RowPtr row_ptr) {
+  uint32_t off[EVEN ? 1 : NI];
+  int step;
+  // bytes(r): row r's distance from the tile's first row, NO_ROW for a row no tile has
+  template <class Bytes> __device__ __forceinline__ void init(int D, Bytes bytes) {
 #pragma unroll
-    for (int i = 0; i < NI; ++i) {
+    for (int i = 0; i < (EVEN ? 1 : NI); ++i) {
       const int id = threadIdx.x + i * NT, r = id / L::CPR, c = id % L::CPR;
-      v[i] = u4{0, 0, 0, 0};
-      if (CH % NT != 0 && id >= CH) continue;
-      const T* p = row_ptr(r);
-      if (p != nullptr && c * L::EPC < D) v[i] = *reinterpret_cast<const u4*>(p + c * L::EPC);
+      const uint32_t b = (CH % NT != 0 && id >= CH) || c * L::EPC >= D ? NO_ROW : bytes(r);
+      off[i] = b == NO_ROW ? b : b + 16 * c;
     }
+    step = EVEN ? (int)bytes(RS) : 0;
+  }
+  // rows 0 .. left - 1 from `first` (uniform over the workgroup)
+  __device__ __forceinline__ void load(const T* first, int left) {
+    const auto rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(first), 0, 0x7fffffff, 0x00020000);
+    const int r = threadIdx.x / L::CPR;
+    // (one load for whole and partial tiles: two alternatives would be merged behind a wait)
+#pragma unroll
+    for (int i = 0; i < NI; ++i)
+      v[i] = __builtin_amdgcn_raw_buffer_load_b128(rsrc, r < left - i * RS ? off[EVEN ? 0 : i] : NO_ROW, i * step, 0);
   }
   __device__ __forceinline__ void store(char* s) const {
 #pragma unroll
@@ -163,6 +181,29 @@ template <class T, int DP, int ROWS, int NT> struct Stage {
     }
   }
 };
+// The operands loaded before a main loop have arrived: said once here, or the compiler's counts, merged
+// over the loop's entries, wait for the prefetched tile before each first product.
+__device__ __forceinline__ void loads_done() { __builtin_amdgcn_s_waitcnt(0x0f70); }   // vmcnt(0)
+
+template <int N> struct Int { static constexpr int value = N; };
+
+// Orders the LDS reads of the N fragment products before it: AHEAD fragments (PER reads each) are in
+// flight before the first product, then each product is followed by the next fragment's reads.
+// (Left to itself the compiler reads, waits and multiplies one fragment at a time.)
+template <int N, int PER, int AHEAD> __device__ __forceinline__ void feed() {
+  constexpr int A = AHEAD < N ? AHEAD : N;
+  __builtin_amdgcn_sched_group_barrier(0x100, A * PER, 0);
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+    if (i + A < N) __builtin_amdgcn_sched_group_barrier(0x100, PER, 0);
+  }
+}
+
+__device__ __forceinline__ float load_f32(const float* base, uint32_t off) {   // base uniform; NO_ROW: 0
+  const auto rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(base), 0, 0x7fffffff, 0x00020000);
+  return __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rsrc, off, 0, 0));
+}
 
 template <class T, int DP> using Frags = typename Ty<T>::Frag[Tile<T, DP>::NCH];
 template <class T, int DP>
@@ -192,29 +233,36 @@ __device__ __forceinline__ void store_col(U* p, const f16v (&o)[DT], float f, in
     }
 }
 
-// the bias of every clamped relative position for one head, log2 domain
+// The bias of every relative position for one head, log2 domain: -R .. R and MARGIN more on either
+// side that repeat the ends, so that a tile which is not wholly beyond +-R reads without clamping.
+constexpr int MARGIN = 64;
+__host__ __device__ __forceinline__ int span_of(int R) { return 2 * (R + MARGIN) + 1; }
 template <class T, int NT>
 __device__ __forceinline__ void load_bias(const Args& a, float* lut, int head) {
   const T* tb = reinterpret_cast<const T*>(a.p.table);
-  for (int i = threadIdx.x; i < 2 * a.p.max_distance + 1; i += NT) {
-    const int b = min(max(a.p.lut[i], 0), a.p.num_buckets - 1);
+  const int R = a.p.max_distance;
+  for (int i = threadIdx.x; i < span_of(R); i += NT) {
+    const int b = min(max(a.p.lut[min(max(i - MARGIN, 0), 2 * R)], 0), a.p.num_buckets - 1);
     lut[i] = (float)tb[(int64_t)b * a.p.Hq + head] * LOG2E;
   }
 }
 
 __device__ __forceinline__ int acc_row(int r, int h) { return 8 * (r >> 2) + 4 * h + (r & 3); }
 
+// a value that is the same in every lane, told to the compiler (scalar registers and branches)
+__device__ __forceinline__ int uni(int x) { return __builtin_amdgcn_readfirstlane(x); }
+
 // where a workgroup's query tile lies
 struct QTile {
-  int seq, pos0, nq, nk, npos, nrows, off, kvh, head0;
+  int pos0, nq, nk, npos, nrows, off, kvh, head0;
   int64_t q0, k0;
   __device__ __forceinline__ QTile(const Args& a, int tile, int hidx) {
-    seq = a.p.q_tiles[2 * tile];
-    pos0 = a.p.q_tiles[2 * tile + 1];
-    q0 = a.p.cu_q[seq];
-    k0 = a.p.cu_k[seq];
-    nq = a.p.cu_q[seq + 1] - (int)q0;
-    nk = a.p.cu_k[seq + 1] - (int)k0;
+    const int seq = uni(a.p.q_tiles[2 * tile]);
+    pos0 = uni(a.p.q_tiles[2 * tile + 1]);
+    q0 = uni(a.p.cu_q[seq]);
+    k0 = uni(a.p.cu_k[seq]);
+    nq = uni(a.p.cu_q[seq + 1]) - (int)q0;
+    nk = uni(a.p.cu_k[seq + 1]) - (int)k0;
     off = nk - nq;
     npos = min(a.p.q_tile, nq - pos0);
     nrows = npos * a.pg;
@@ -226,15 +274,18 @@ struct QTile {
   }
 };
 
-// scores of one 32x32 tile to log2-domain values with bias: s c + bias
-template <int N>
-__device__ __forceinline__ void add_bias(f16v& s, float c, const float* lut, int rel0, int h, int R, int sign) {
-  // relative position of register r: rel0 + sign * acc_row(r, h)
-  (void)N;
+// scores of one 32x32 tile to the log2 domain with bias, s c + bias.  Register r's relative position is
+// rel0 + SIGN acc_row(r, h); lo .. hi (uniform) bounds those of the tile.
+template <int SIGN>
+__device__ __forceinline__ void add_bias(f16v& s, float c, const float* lut, int rel0, int lo, int hi, int h, int R) {
+  if (hi <= -R || lo >= R) {                               // one bucket for the whole tile
+    const float b = lut[hi <= -R ? 0 : 2 * (R + MARGIN)];
 #pragma unroll
-  for (int r = 0; r < 16; ++r) {
-    const int rel = rel0 + sign * acc_row(r, h);
-    s[r] = fmaf(s[r], c, lut[min(max(rel, -R), R) + R]);
+    for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], c, b);
+  } else {
+    const float* p = lut + (rel0 + SIGN * 4 * h + R + MARGIN);
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], c, p[SIGN * acc_row(r, 0)]);
   }
 }
 
@@ -242,12 +293,17 @@ __device__ __forceinline__ void add_bias(f16v& s, float c, const float* lut, int
 // forward
 // -------------------------------------------------------------------------------------------
 template <class T, int DP> constexpr int key_tile() { return sizeof(T) == 2 ? 64 : 32; }
-// waves per SIMD the registers are budgeted for: fp32 at head_dim 128 holds two operands of 64
-// registers beside 64 of sums, and takes the whole file
-template <class T, int DP> constexpr int occ() { return sizeof(T) == 4 && DP == 128 ? 1 : 2; }
+// waves per SIMD the registers are budgeted for.  One (all 512 registers) where two would spill: dK /
+// dV at head_dim 128 hold 128 registers of sums beside 64 of operands (two waves, spilling: 1.50 ms,
+// one: 0.73 ms, causal training step of 10 k tokens, 16 heads over 4), fp32 twice the operands,
+// and two-wave workgroups stage twice as much per thread (their LDS allows one wave per SIMD anyway).
+template <class T, int DP, bool BIAS, int NW, bool DQ> constexpr int occ() {
+  return DP == 128 && (sizeof(T) == 4 || NW == 2 || (DQ && BIAS)) ? 1 : 2;
+}
+template <class T, int DP> constexpr int occ_kv() { return DP == 128 || (sizeof(T) == 4 && DP == 64) ? 1 : 2; }
 
 template <class T, int DP, bool BIAS, int NW>
-__global__ __launch_bounds__(NW * 64, (occ<T, DP>())) void fwd_kernel(Args a) {
+__global__ __launch_bounds__(NW * 64, (occ<T, DP, BIAS, NW, false>())) void fwd_kernel(Args a) {
   using L = Tile<T, DP>;
   constexpr int NT = NW * 64, BN = key_tile<T, DP>(), NB = BN / 32, TILE = BN * L::RB;
   extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -255,17 +311,17 @@ __global__ __launch_bounds__(NW * 64, (occ<T, DP>())) void fwd_kernel(Args a) {
   const int nh = a.p.Hkv * a.nsub;
   const int hidx = blockIdx.x % nh;
   const QTile t(a, blockIdx.x / nh, hidx);
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, h = lane >> 5, D = a.p.D, R = a.p.max_distance;
+  const int lane = threadIdx.x & 63, w = uni(threadIdx.x >> 6), h = lane >> 5, D = a.p.D, R = a.p.max_distance;
   if (BIAS) load_bias<T, NT>(a, lut, t.head0);
 
   const int row = w * 32 + (lane & 31), dpos = div_pg(a, row);
   const bool valid = row < t.nrows;
   const int head = t.head0 + row - dpos * a.pg;
   const int lim = valid ? t.limit(a, row) : t.nk;
-  const int qabs = t.pos0 + dpos + t.off;
+  const int qfirst = t.pos0 + w * 32 + t.off, qabs = t.pos0 + dpos + t.off;   // (a bias: one head per tile, row = position)
   const bool active = w * 32 < t.nrows;
-  const int wmin = t.limit(a, w * 32), wmax = active ? t.limit(a, min(w * 32 + 31, t.nrows - 1)) : 0;
-  const int kend = t.limit(a, t.nrows - 1);
+  const int wmin = uni(t.limit(a, w * 32)), wmax = active ? uni(t.limit(a, min(w * 32 + 31, t.nrows - 1))) : 0;
+  const int kend = uni(t.limit(a, t.nrows - 1));
   const int nt = (kend + BN - 1) / BN, per = (nt + a.nsplit - 1) / a.nsplit;
   const int t0 = blockIdx.y * per, t1 = min(nt, t0 + per);
 
@@ -280,19 +336,22 @@ __global__ __launch_bounds__(NW * 64, (occ<T, DP>())) void fwd_kernel(Args a) {
 
   const T* kb = reinterpret_cast<const T*>(a.p.k) + t.k0 * a.p.k_ts + t.kvh * a.p.k_hs;
   const T* vb = reinterpret_cast<const T*>(a.p.v) + t.k0 * a.p.v_ts + t.kvh * a.p.v_hs;
-  Stage<T, DP, BN, NT> ks, vs;
+  Stage<T, DP, BN, NT, true> ks, vs;
+  ks.init(D, [&](int r) { return (uint32_t)r * (uint32_t)(a.p.k_ts * sizeof(T)); });
+  vs.init(D, [&](int r) { return (uint32_t)r * (uint32_t)(a.p.v_ts * sizeof(T)); });
   auto fetch = [&](int j) {
-    ks.load(D, [&](int r) { const int key = j * BN + r; return key < t.nk ? kb + key * a.p.k_ts : nullptr; });
-    vs.load(D, [&](int r) { const int key = j * BN + r; return key < t.nk ? vb + key * a.p.v_ts : nullptr; });
+    ks.load(kb + (int64_t)j * BN * a.p.k_ts, t.nk - j * BN);
+    vs.load(vb + (int64_t)j * BN * a.p.v_ts, t.nk - j * BN);
   };
   if (t0 < t1) {
     fetch(t0);
     ks.store(smem);
     vs.store(smem + TILE);
   }
+  loads_done();
   __syncthreads();
-  for (int j = t0; j < t1; ++j) {
-    const char* K = smem + ((j - t0) & 1) * 2 * TILE;
+  auto step = [&](int j, auto buf) {
+    const char* K = smem + buf.value * 2 * TILE;
     const char* V = K + TILE;
     if (j + 1 < t1) fetch(j + 1);
     const int base = j * BN;
@@ -304,11 +363,13 @@ __global__ __launch_bounds__(NW * 64, (occ<T, DP>())) void fwd_kernel(Args a) {
 #pragma unroll
         for (int k = 0; k < L::NCH; ++k) s[n] = mma(L::row(K, 32 * n + (lane & 31), k, h), qf[k], s[n]);
       }
+      feed<NB * L::NCH, 1, 4>();
       // scores to the units of the running maximum: raw without a bias, log2 with one
       const float c = BIAS ? 1.f : a.c;
       if (BIAS) {
 #pragma unroll
-        for (int n = 0; n < NB; ++n) add_bias<0>(s[n], a.c, lut, base + 32 * n - qabs, h, R, 1);
+        for (int n = 0; n < NB; ++n)
+          add_bias<1>(s[n], a.c, lut, base + 32 * n - qabs, base + 32 * n - qfirst - 31, base + 32 * n - qfirst + 31, h, R);
       }
       if (base + BN > wmin) {
 #pragma unroll
@@ -349,13 +410,18 @@ __global__ __launch_bounds__(NW * 64, (occ<T, DP>())) void fwd_kernel(Args a) {
 #pragma unroll
           for (int dt = 0; dt < L::DT; ++dt) o[dt] = mma(L::col(V, 32 * n, b, dt, lane), pf, o[dt]);
         }
+      feed<NB * L::TB * L::DT, L::CR, 3>();
     }
     if (j + 1 < t1) {
-      char* Kn = smem + ((j + 1 - t0) & 1) * 2 * TILE;
+      char* Kn = smem + (1 - buf.value) * 2 * TILE;
       ks.store(Kn);
       vs.store(Kn + TILE);
     }
     __syncthreads();
+  };
+  for (int j = t0; j < t1; j += 2) {
+    step(j, Int<0>{});
+    if (j + 1 < t1) step(j + 1, Int<1>{});
   }
   l = xsum32(l);
   if (!valid) return;
@@ -421,32 +487,32 @@ __device__ __forceinline__ float pow2_of(uint32_t bits) {   // 2^e of |x|, 1 for
 }
 
 template <class T, int DP, bool BIAS, int NW>
-__global__ __launch_bounds__(NW * 64, (occ<T, DP>())) void dq_kernel(Args a) {
+__global__ __launch_bounds__(NW * 64, (occ<T, DP, BIAS, NW, true>())) void dq_kernel(Args a) {
   using L = Tile<T, DP>;
   constexpr int NT = NW * 64, BN = key_tile<T, DP>(), NB = BN / 32, TILE = BN * L::RB;
   constexpr bool HALF = __is_same(T, _Float16);
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int R = a.p.max_distance, NH = 2 * R + 1;
   float* lut = reinterpret_cast<float*>(smem + 4 * TILE);
-  float* hist = lut + NH + (threadIdx.x >> 6) * NH;            // this wave's sums by relative position
+  float* hist = lut + span_of(R) * (1 + (threadIdx.x >> 6));   // this wave's sums by relative position
   const int nh = a.p.Hkv * a.nsub;
   const int hidx = blockIdx.x % nh;
   const QTile t(a, blockIdx.x / nh, hidx);
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, h = lane >> 5, D = a.p.D;
+  const int lane = threadIdx.x & 63, w = uni(threadIdx.x >> 6), h = lane >> 5, D = a.p.D;
   const bool sums = BIAS && a.p.dtable != nullptr;
   if (BIAS) load_bias<T, NT>(a, lut, t.head0);
   if (sums)
-    for (int i = lane; i < NH; i += 64) hist[i] = 0.f;
+    for (int i = lane; i < span_of(R); i += 64) hist[i] = 0.f;
 
   const int row = w * 32 + (lane & 31), dpos = div_pg(a, row);
   const bool valid = row < t.nrows;
   const int head = t.head0 + row - dpos * a.pg;
   const int lim = valid ? t.limit(a, row) : 0;
-  const int qabs = t.pos0 + dpos + t.off;
+  const int qfirst = t.pos0 + w * 32 + t.off, qabs = t.pos0 + dpos + t.off;   // (a bias: one head per tile, row = position)
   const bool active = w * 32 < t.nrows;
-  const int wmin = w * 32 + 31 < t.nrows ? t.limit(a, w * 32) : 0;
-  const int wmax = active ? t.limit(a, min(w * 32 + 31, t.nrows - 1)) : 0;
-  const int kend = t.limit(a, t.nrows - 1);
+  const int wmin = w * 32 + 31 < t.nrows ? uni(t.limit(a, w * 32)) : 0;
+  const int wmax = active ? uni(t.limit(a, min(w * 32 + 31, t.nrows - 1))) : 0;
+  const int kend = uni(t.limit(a, t.nrows - 1));
   const int nt = (kend + BN - 1) / BN, per = (nt + a.nsplit - 1) / a.nsplit;
   const int t0 = blockIdx.y * per, t1 = min(nt, t0 + per);
 
@@ -487,19 +553,22 @@ __global__ __launch_bounds__(NW * 64, (occ<T, DP>())) void dq_kernel(Args a) {
 
   const T* kb = reinterpret_cast<const T*>(a.p.k) + t.k0 * a.p.k_ts + t.kvh * a.p.k_hs;
   const T* vb = reinterpret_cast<const T*>(a.p.v) + t.k0 * a.p.v_ts + t.kvh * a.p.v_hs;
-  Stage<T, DP, BN, NT> ks, vs;
+  Stage<T, DP, BN, NT, true> ks, vs;
+  ks.init(D, [&](int r) { return (uint32_t)r * (uint32_t)(a.p.k_ts * sizeof(T)); });
+  vs.init(D, [&](int r) { return (uint32_t)r * (uint32_t)(a.p.v_ts * sizeof(T)); });
   auto fetch = [&](int j) {
-    ks.load(D, [&](int r) { const int key = j * BN + r; return key < t.nk ? kb + key * a.p.k_ts : nullptr; });
-    vs.load(D, [&](int r) { const int key = j * BN + r; return key < t.nk ? vb + key * a.p.v_ts : nullptr; });
+    ks.load(kb + (int64_t)j * BN * a.p.k_ts, t.nk - j * BN);
+    vs.load(vb + (int64_t)j * BN * a.p.v_ts, t.nk - j * BN);
   };
   if (t0 < t1) {
     fetch(t0);
     ks.store(smem);
     vs.store(smem + TILE);
   }
+  loads_done();
   __syncthreads();
-  for (int j = t0; j < t1; ++j) {
-    const char* K = smem + ((j - t0) & 1) * 2 * TILE;
+  auto step = [&](int j, auto buf) {
+    const char* K = smem + buf.value * 2 * TILE;
     const char* V = K + TILE;
     if (j + 1 < t1) fetch(j + 1);
 #pragma unroll
@@ -511,9 +580,11 @@ __global__ __launch_bounds__(NW * 64, (occ<T, DP>())) void dq_kernel(Args a) {
         for (int k = 0; k < L::NCH; ++k) s = mma(L::row(K, 32 * n + (lane & 31), k, h), qf[k], s);
 #pragma unroll
         for (int k = 0; k < L::NCH; ++k) g = mma(L::row(V, 32 * n + (lane & 31), k, h), gf[k], g);
+        feed<2 * L::NCH, 1, 4>();
         const float c = BIAS ? 1.f : a.c;
         const int rel0 = base - qabs;
-        if (BIAS) add_bias<0>(s, a.c, lut, rel0, h, R, 1);
+        const int lo = base - qfirst - 31, hi = base - qfirst + 31;   // the tile's relative positions
+        if (BIAS) add_bias<1>(s, a.c, lut, rel0, lo, hi, h, R);
 #pragma unroll
         for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c, -lse)) * (g[r] - delta);
         if (base + 32 > wmin) {
@@ -522,8 +593,6 @@ __global__ __launch_bounds__(NW * 64, (occ<T, DP>())) void dq_kernel(Args a) {
             if (base + acc_row(r, h) >= lim) s[r] = 0.f;
         }
         if (sums) {
-          // wave-uniform: the tile lies beyond +-R for every row (row 0's and row 31's distances)
-          const int lo = base - (t.pos0 + w * 32 + 31 + t.off), hi = base + 31 - (t.pos0 + w * 32 + t.off);
           if (hi <= -R) {
 #pragma unroll
             for (int r = 0; r < 16; ++r) far_lo += s[r];
@@ -534,20 +603,12 @@ __global__ __launch_bounds__(NW * 64, (occ<T, DP>())) void dq_kernel(Args a) {
             // one half of the wave at a time: the 32 lanes of a half meet 32 different distances in
             // each register and a wave's LDS operations keep their order, so every sum of this
             // wave-private array is taken in one fixed order
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-              const int rel = rel0 + acc_row(r, h);
-              if (rel <= -R) far_lo += s[r];
-              else if (rel >= R) far_hi += s[r];
-            }
+            float* p = hist + (rel0 + 4 * h + R + MARGIN);
             for (int half = 0; half < 2; ++half) {
               if (h == half) {
 #pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                  const int rel = rel0 + acc_row(r, h);
-                  if (rel > -R && rel < R)
-                    __hip_atomic_fetch_add(hist + rel + R, s[r], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WAVEFRONT);
-                }
+                for (int r = 0; r < 16; ++r)
+                  __hip_atomic_fetch_add(p + acc_row(r, 0), s[r], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WAVEFRONT);
               }
             }
           }
@@ -562,28 +623,38 @@ __global__ __launch_bounds__(NW * 64, (occ<T, DP>())) void dq_kernel(Args a) {
 #pragma unroll
           for (int dt = 0; dt < L::DT; ++dt) o[dt] = mma(L::col(K, 32 * n, b, dt, lane), sf, o[dt]);
         }
+        feed<L::TB * L::DT, L::CR, 3>();
       }
     }
     if (j + 1 < t1) {
-      char* Kn = smem + ((j + 1 - t0) & 1) * 2 * TILE;
+      char* Kn = smem + (1 - buf.value) * 2 * TILE;
       ks.store(Kn);
       vs.store(Kn + TILE);
     }
     __syncthreads();
+  };
+  for (int j = t0; j < t1; j += 2) {
+    step(j, Int<0>{});
+    if (j + 1 < t1) step(j + 1, Int<1>{});
   }
   if (sums) {
+    // the margins belong to the two ends
+    for (int i = lane; i <= MARGIN; i += 64) {
+      far_lo += hist[i];
+      far_hi += hist[2 * R + MARGIN + i];
+    }
     far_lo = wave_sum(far_lo);
     far_hi = wave_sum(far_hi);
     if (lane == 0) {
-      hist[0] = far_lo;
-      hist[2 * R] += far_hi;                                   // R >= 1: its own slot
+      hist[MARGIN] = far_lo;
+      hist[2 * R + MARGIN] = far_hi;                           // (R >= 1: not the same place)
     }
     __syncthreads();
     float* out = a.hist + ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * NH;
     for (int i = threadIdx.x; i < NH; i += NT) {
       float x = 0.f;
 #pragma unroll
-      for (int v = 0; v < NW; ++v) x += lut[NH + v * NH + i];
+      for (int v = 0; v < NW; ++v) x += lut[(1 + v) * span_of(R) + MARGIN + i];
       out[i] = x;
     }
   }
@@ -596,21 +667,17 @@ __global__ __launch_bounds__(NW * 64, (occ<T, DP>())) void dq_kernel(Args a) {
 // sums by relative position of the n workgroups of a head (workgroup i * Hq + head), 16 slices of
 // them in order, then the slices in order: rel[head][NH]
 __global__ __launch_bounds__(1024) void hist_sum_kernel(const float* hist, int n, int Hq, int NH, float* rel);
-// dtable[b][head] = sum of rel[head][i] over the relative positions i of bucket b, in order
+// dtable[b][head] = sum of rel[head][i] over the relative positions i of bucket b: a wave per bucket,
+// each lane its positions in order, then the lanes (one thread per bucket took 15 us)
 template <class T>
-__global__ __launch_bounds__(256) void hist_bucket_kernel(const float* rel, const int32_t* lut, int NH, int Hq, int nb,
-                                                          T* dtable) {
-  extern __shared__ float sm[];
-  int* bucket = reinterpret_cast<int*>(sm + NH);
-  for (int i = threadIdx.x; i < NH; i += 256) {
-    sm[i] = rel[(int64_t)blockIdx.x * NH + i];
-    bucket[i] = min(max(lut[i], 0), nb - 1);
-  }
-  __syncthreads();
-  for (int b = threadIdx.x; b < nb; b += 256) {
+__global__ __launch_bounds__(1024) void hist_bucket_kernel(const float* rel, const int32_t* lut, int NH, int Hq, int nb,
+                                                           T* dtable) {
+  const int lane = threadIdx.x & 63;
+  for (int b = threadIdx.x >> 6; b < nb; b += 16) {
     float x = 0.f;
-    for (int i = 0; i < NH; ++i) x += bucket[i] == b ? sm[i] : 0.f;
-    dtable[(int64_t)b * Hq + blockIdx.x] = (T)x;
+    for (int i = lane; i < NH; i += 64) x += min(max(lut[i], 0), nb - 1) == b ? rel[(int64_t)blockIdx.x * NH + i] : 0.f;
+    x = wave_sum(x);
+    if (lane == 0) dtable[(int64_t)b * Hq + blockIdx.x] = (T)x;
   }
 }
 
@@ -618,7 +685,7 @@ __global__ __launch_bounds__(256) void hist_bucket_kernel(const float* rel, cons
 // backward: dK, dV
 // -------------------------------------------------------------------------------------------
 template <class T, int DP, bool BIAS, int NW>
-__global__ __launch_bounds__(NW * 64, (occ<T, DP>())) void dkv_kernel(Args a) {
+__global__ __launch_bounds__(NW * 64, (occ_kv<T, DP>())) void dkv_kernel(Args a) {
   using L = Tile<T, DP>;
   constexpr int NT = NW * 64, BQ = key_tile<T, DP>(), NB = BQ / 32, TILE = BQ * L::RB;
   constexpr bool HALF = __is_same(T, _Float16);
@@ -626,10 +693,10 @@ __global__ __launch_bounds__(NW * 64, (occ<T, DP>())) void dkv_kernel(Args a) {
   float* stat = reinterpret_cast<float*>(smem + 4 * TILE);     // [2][lse BQ | delta BQ]
   float* lut = stat + 4 * BQ;
   const int kvh = blockIdx.x % a.p.Hkv, tile = blockIdx.x / a.p.Hkv, D = a.p.D, R = a.p.max_distance;
-  const int seq = a.p.k_tiles[2 * tile], key0 = a.p.k_tiles[2 * tile + 1];
-  const int64_t q0 = a.p.cu_q[seq], k0 = a.p.cu_k[seq];
-  const int nq = a.p.cu_q[seq + 1] - (int)q0, nk = a.p.cu_k[seq + 1] - (int)k0, off = nk - nq;
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, h = lane >> 5;
+  const int seq = uni(a.p.k_tiles[2 * tile]), key0 = uni(a.p.k_tiles[2 * tile + 1]);
+  const int64_t q0 = uni(a.p.cu_q[seq]), k0 = uni(a.p.cu_k[seq]);
+  const int nq = uni(a.p.cu_q[seq + 1]) - (int)q0, nk = uni(a.p.cu_k[seq + 1]) - (int)k0, off = nk - nq;
+  const int lane = threadIdx.x & 63, w = uni(threadIdx.x >> 6), h = lane >> 5;
   const int key = key0 + w * 32 + (lane & 31);
   const bool valid = key < nk;
   typename Ty<T>::Frag kf[L::NCH], vf[L::NCH];
@@ -643,10 +710,10 @@ __global__ __launch_bounds__(NW * 64, (occ<T, DP>())) void dkv_kernel(Args a) {
   const float down = 1.f / up;
 
   // rows (position * PG + head) that see any of the tile's keys, tile by tile, one head group after
-  // the other: it = sub * ntq + row tile
-  const int nrows = nq * a.pg;
-  const int first = a.p.causal ? min(max(key0 - off, 0), nq) * a.pg / BQ : 0;
-  const int ntq = max((nrows + BQ - 1) / BQ - first, 0), total = a.nsub * ntq;
+  // the other: it = sub * ntq + row tile.  A row tile holds whole positions: BP of them, BP PG rows.
+  const int bp = BQ / a.pg, br = bp * a.pg, nrows = nq * a.pg;
+  const int first = a.p.causal ? min(max(key0 - off, 0), nq) / bp : 0;
+  const int ntq = max((nq + bp - 1) / bp - first, 0), total = a.nsub * ntq;
   const int per = (total + a.nsplit - 1) / a.nsplit, t0 = blockIdx.y * per, t1 = min(total, t0 + per);
   // the first row that sees this lane's key / the wave's first and last key
   const int see = a.p.causal ? (key - off) * a.pg : 0;
@@ -654,36 +721,34 @@ __global__ __launch_bounds__(NW * 64, (occ<T, DP>())) void dkv_kernel(Args a) {
   const int wlast = a.p.causal ? (key0 + w * 32 + 31 - off) * a.pg : 0;
   const bool active = key0 + w * 32 < nk;
 
-  Stage<T, DP, BQ, NT> qs, gs;
-  float st_l = INF, st_d = 0.f;
-  auto fetch = [&](int it) {
-    const int sub = it / ntq, rb = (first + it - sub * ntq) * BQ;
-    const int head0 = kvh * a.group + sub * a.pg;
-    auto ptr = [&](const void* x, int64_t ts, int64_t hs, int r) -> const T* {
-      const int rr = rb + r;
-      if (rr >= nrows) return nullptr;
-      const int pos = div_pg(a, rr);
-      return reinterpret_cast<const T*>(x) + (q0 + pos) * ts + (int64_t)(head0 + rr - pos * a.pg) * hs;
+  Stage<T, DP, BQ, NT, false> qs, gs;
+  float st_l, st_d;
+  bool st_in;
+  auto bytes = [&](int64_t ts, int64_t hs) {
+    return [=](int r) {
+      const int pos = div_pg(a, r);
+      return r >= br ? NO_ROW : (uint32_t)((pos * ts + (r - pos * a.pg) * hs) * (int)sizeof(T));
     };
-    qs.load(D, [&](int r) { return ptr(a.p.q, a.p.q_ts, a.p.q_hs, r); });
-    gs.load(D, [&](int r) { return ptr(a.p.dout, a.p.do_ts, a.p.do_hs, r); });
-    if (threadIdx.x < BQ) {
-      const int rr = rb + threadIdx.x;
-      st_l = INF;
-      st_d = 0.f;
-      if (rr < nrows) {
-        const int pos = div_pg(a, rr);
-        const int64_t rid = (q0 + pos) * a.p.Hq + head0 + rr - pos * a.pg;
-        st_l = a.p.lse[rid];
-        st_d = a.delta[rid];
-      }
-    }
+  };
+  qs.init(D, bytes(a.p.q_ts, a.p.q_hs));
+  gs.init(D, bytes(a.p.do_ts, a.p.do_hs));
+  const int spos = div_pg(a, threadIdx.x), sofs = spos * a.p.Hq + (int)threadIdx.x - spos * a.pg;
+  auto fetch = [&](int it) {
+    const int sub = it / ntq, pos = (first + it - sub * ntq) * bp, head0 = kvh * a.group + sub * a.pg;
+    const int left = min(nrows - pos * a.pg, br);
+    qs.load(reinterpret_cast<const T*>(a.p.q) + (q0 + pos) * a.p.q_ts + head0 * a.p.q_hs, left);
+    gs.load(reinterpret_cast<const T*>(a.p.dout) + (q0 + pos) * a.p.do_ts + head0 * a.p.do_hs, left);
+    const int64_t rid = (q0 + pos) * a.p.Hq + head0;
+    const uint32_t at = (int)threadIdx.x < left ? 4u * sofs : NO_ROW;
+    st_l = load_f32(a.p.lse + rid, at);
+    st_d = load_f32(a.delta + rid, at);
+    st_in = (int)threadIdx.x < left;
   };
   auto commit = [&](int b) {
     qs.store(smem + b * 2 * TILE);
     gs.store(smem + b * 2 * TILE + TILE);
     if (threadIdx.x < BQ) {
-      stat[b * 2 * BQ + threadIdx.x] = st_l;
+      stat[b * 2 * BQ + threadIdx.x] = st_in ? st_l : INF;
       stat[b * 2 * BQ + BQ + threadIdx.x] = st_d;
     }
   };
@@ -692,14 +757,15 @@ __global__ __launch_bounds__(NW * 64, (occ<T, DP>())) void dkv_kernel(Args a) {
     fetch(t0);
     commit(0);
   }
+  loads_done();
   __syncthreads();
-  for (int it = t0; it < t1; ++it) {
-    const int b = (it - t0) & 1;
+  auto step = [&](int it, auto buf) {
+    constexpr int b = buf.value;
     const char* Q = smem + b * 2 * TILE;
     const char* G = Q + TILE;
     const float* lse = stat + b * 2 * BQ;
     const float* dl = lse + BQ;
-    const int sub = it / ntq, rb = (first + it - sub * ntq) * BQ;
+    const int sub = it / ntq, rb = (first + it - sub * ntq) * br;
     if (BIAS && sub != sub_now) {                              // the next head's biases
       __syncthreads();
       load_bias<T, NT>(a, lut, kvh * a.group + sub * a.pg);
@@ -707,50 +773,64 @@ __global__ __launch_bounds__(NW * 64, (occ<T, DP>())) void dkv_kernel(Args a) {
       sub_now = sub;
     }
     if (it + 1 < t1) fetch(it + 1);
+    if (active && rb + BQ > wfirst) {
+      f16v s[NB], g[NB];
 #pragma unroll
-    for (int n = 0; n < NB; ++n) {
-      const int base = rb + 32 * n;
-      if (active && base < nrows && base + 31 >= wfirst) {
-        f16v s = f16v{}, g = f16v{};
+      for (int n = 0; n < NB; ++n) {
+        s[n] = f16v{};
+        g[n] = f16v{};
 #pragma unroll
-        for (int k = 0; k < L::NCH; ++k) s = mma(L::row(Q, 32 * n + (lane & 31), k, h), kf[k], s);
-        if (BIAS) add_bias<0>(s, a.c, lut, key - off - base, h, R, -1);
-        const float c = BIAS ? 1.f : a.c;
+        for (int k = 0; k < L::NCH; ++k) s[n] = mma(L::row(Q, 32 * n + (lane & 31), k, h), kf[k], s[n]);
+#pragma unroll
+        for (int k = 0; k < L::NCH; ++k) g[n] = mma(L::row(G, 32 * n + (lane & 31), k, h), vf[k], g[n]);
+      }
+      feed<2 * NB * L::NCH, 1, 4>();
+      const float c = BIAS ? 1.f : a.c;
+#pragma unroll
+      for (int n = 0; n < NB; ++n) {
+        if (BIAS) {
+          const int lo = key0 + w * 32 - off - rb - 32 * n - 31;
+          add_bias<-1>(s[n], a.c, lut, key - off - rb - 32 * n, lo, lo + 62, h, R);
+        }
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
           const f4 x = *reinterpret_cast<const f4*>(lse + 32 * n + 8 * q + 4 * h);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) s[4 * q + e] = __builtin_amdgcn_exp2f(fmaf(s[4 * q + e], c, -x[e]));
+          for (int e = 0; e < 4; ++e) s[n][4 * q + e] = __builtin_amdgcn_exp2f(fmaf(s[n][4 * q + e], c, -x[e]));
         }
-        if (base < wlast) {
+        if (rb + 32 * n < wlast) {
 #pragma unroll
           for (int r = 0; r < 16; ++r)
-            if (base + acc_row(r, h) < see) s[r] = 0.f;
+            if (rb + 32 * n + acc_row(r, h) < see) s[n][r] = 0.f;
         }
 #pragma unroll
         for (int t = 0; t < L::TB; ++t) {
-          const auto pf = take<T>(s, t);
+          const auto pf = take<T>(s[n], t);
 #pragma unroll
           for (int dt = 0; dt < L::DT; ++dt) dv[dt] = mma(L::col(G, 32 * n, t, dt, lane), pf, dv[dt]);
         }
-#pragma unroll
-        for (int k = 0; k < L::NCH; ++k) g = mma(L::row(G, 32 * n + (lane & 31), k, h), vf[k], g);
+        feed<L::DT * L::TB, L::CR, 3>();
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
           const f4 x = *reinterpret_cast<const f4*>(dl + 32 * n + 8 * q + 4 * h);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) s[4 * q + e] *= (g[4 * q + e] - x[e]) * (HALF ? down : 1.f);
+          for (int e = 0; e < 4; ++e) s[n][4 * q + e] *= (g[n][4 * q + e] - x[e]) * (HALF ? down : 1.f);
         }
 #pragma unroll
         for (int t = 0; t < L::TB; ++t) {
-          const auto sf = take<T>(s, t);
+          const auto sf = take<T>(s[n], t);
 #pragma unroll
           for (int dt = 0; dt < L::DT; ++dt) dk[dt] = mma(L::col(Q, 32 * n, t, dt, lane), sf, dk[dt]);
         }
+        feed<L::DT * L::TB, L::CR, 3>();
       }
     }
     if (it + 1 < t1) commit(1 - b);
     __syncthreads();
+  };
+  for (int it = t0; it < t1; it += 2) {
+    step(it, Int<0>{});
+    if (it + 1 < t1) step(it + 1, Int<1>{});
   }
   if (!valid) return;
   const int64_t rid = (k0 + key) * a.p.Hkv + kvh, rows = a.p.total_k * a.p.Hkv;
@@ -787,7 +867,7 @@ template <class T, int DP, bool BIAS> int fwd_dp(const Plan& p, hipStream_t s) {
   Args a = p.a;
   a.nsplit = p.split_q;
   const int wgs = a.p.n_q_tiles * a.p.Hkv * a.nsub;
-  const size_t lds = 4 * key_tile<T, DP>() * Tile<T, DP>::RB + (BIAS ? (2 * a.p.max_distance + 1) * 4 : 0);
+  const size_t lds = 4 * key_tile<T, DP>() * Tile<T, DP>::RB + (BIAS ? span_of(a.p.max_distance) * 4 : 0);
   const int rc = p.nwq == 2 ? launch<T>(fwd_kernel<T, DP, BIAS, 2>, dim3(wgs, a.nsplit), 128, lds, a, s)
                             : launch<T>(fwd_kernel<T, DP, BIAS, 4>, dim3(wgs, a.nsplit), 256, lds, a, s);
   if (rc || a.nsplit == 1) return rc;
@@ -811,7 +891,7 @@ template <class T, int DP, bool BIAS> int bwd_dp(const Plan& p, hipStream_t s) {
   if (a.p.n_q_tiles > 0) {
     a.nsplit = p.split_q;
     const int wgs = a.p.n_q_tiles * a.p.Hkv * a.nsub;
-    const size_t lds = 4 * BN * RB + (BIAS ? (1 + p.nwq) * NH * 4 : 0);
+    const size_t lds = 4 * BN * RB + (BIAS ? (1 + p.nwq) * span_of(a.p.max_distance) * 4 : 0);
     const int rc = p.nwq == 2 ? launch<T>(dq_kernel<T, DP, BIAS, 2>, dim3(wgs, a.nsplit), 128, lds, a, s)
                               : launch<T>(dq_kernel<T, DP, BIAS, 4>, dim3(wgs, a.nsplit), 256, lds, a, s);
     if (rc) return rc;
@@ -827,13 +907,13 @@ template <class T, int DP, bool BIAS> int bwd_dp(const Plan& p, hipStream_t s) {
     hipLaunchKernelGGL(hist_sum_kernel, dim3((NH + 63) / 64, a.p.Hq), dim3(1024), 0, s, a.hist,
                        a.p.n_q_tiles * p.split_q, a.p.Hq, NH, rel);
     VAESNE_CHECK_LAUNCH();
-    hipLaunchKernelGGL((hist_bucket_kernel<T>), dim3(a.p.Hq), dim3(256), NH * 8, s, rel, a.p.lut, NH, a.p.Hq,
+    hipLaunchKernelGGL((hist_bucket_kernel<T>), dim3(a.p.Hq), dim3(1024), 0, s, rel, a.p.lut, NH, a.p.Hq,
                        a.p.num_buckets, reinterpret_cast<T*>(a.p.dtable));
     VAESNE_CHECK_LAUNCH();
   }
   if (a.p.n_k_tiles == 0) return 0;
   a.nsplit = p.split_k;
-  const size_t lds = 4 * BN * RB + 16 * BN + (BIAS ? NH * 4 : 0);
+  const size_t lds = 4 * BN * RB + 16 * BN + (BIAS ? span_of(a.p.max_distance) * 4 : 0);
   const int wgs = a.p.n_k_tiles * a.p.Hkv;
   const int rc = p.nwk == 2 ? launch<T>(dkv_kernel<T, DP, BIAS, 2>, dim3(wgs, a.nsplit), 128, lds, a, s)
                             : launch<T>(dkv_kernel<T, DP, BIAS, 4>, dim3(wgs, a.nsplit), 256, lds, a, s);

@@ -42,18 +42,26 @@ namespace {
 constexpr int SLOTS = 512;            // workgroups the chip runs at once: two of 64 KB LDS per CU
 constexpr int MAX_SPLIT = 64;
 constexpr int64_t MAX_PART = 256 << 20;
+constexpr int64_t MAX_STRIDE = 1 << 22;  // elements: a tile of 64 rows spans less than 2^31 bytes
 constexpr int64_t MAX_ROWS = 1 << 25; // rows of one sequence: 32-bit row arithmetic with room
 
 // Parts to cut the streamed axis into.  Each of `wgs` workgroups walks up to `longest` tiles, `mean` on
-// average.  A part shorter than 4 tiles costs more in joining than it saves; one longer than twice
-// the chip's mean share leaves the other CUs idle at the end.
-int splits(int64_t wgs, int64_t longest, double mean, int64_t part_bytes) {
-  const double share = std::max(4.0, wgs * mean / SLOTS);
-  if (longest < 1.5 * share) return 1;
-  int64_t n = (int64_t)((longest + share - 1) / share);
-  n = std::min<int64_t>(n, MAX_SPLIT);
-  n = std::min<int64_t>(n, std::max<int64_t>(1, MAX_PART / std::max<int64_t>(part_bytes, 1)));
-  return (int)std::max<int64_t>(n, 1);
+// average; `slots` of them run at once, longest first.  A part costs about six tiles more (its own
+// loads, its sums to memory and their joining), so the end of the launch is estimated as
+//   (all tiles and parts) / slots + half of the longest part, at least the longest part,
+// eight tiles more for the joining launch, and the cheapest count of parts of 4 tiles or more taken.  (fp16 training, 6 sequences of up to 2047, 12 heads: one part 48 us
+// forward, two 58 + 17 us; dK / dV of the bf16 training step: one part 873 us, two 680 + 22 us.)
+int splits(int64_t wgs, int64_t longest, double mean, int64_t part_bytes, int slots) {
+  const double over = 6, join = 8;
+  const int64_t most = std::min<int64_t>(std::min<int64_t>(MAX_SPLIT, longest / 4), MAX_PART / std::max<int64_t>(part_bytes, 1));
+  int best = 1;
+  double least = 0;
+  for (int n = 1; n <= std::max<int64_t>(most, 1); ++n) {
+    const double own = (double)((longest + n - 1) / n) + over;
+    const double end = std::max(wgs * (mean + n * over) / slots + 0.5 * own, own) + (n > 1 ? join : 0);
+    if (n == 1 || end < least) { best = n; least = end; }
+  }
+  return best;
 }
 
 int64_t up16(int64_t n) { return (n + 15) & ~(int64_t)15; }
@@ -94,9 +102,10 @@ int make_plan(const vaesne_packed_attn* a, Plan* p) {
   const int64_t qrows = a->total_q * a->Hq, krows = a->total_k * a->Hkv;
   const double n = std::max(a->nseq, 1);
   p->split_q = splits((int64_t)a->n_q_tiles * a->Hkv * p->a.nsub, (a->max_k + bn - 1) / bn, a->total_k / n / bn,
-                      qrows * (a->D + 1) * 4);
-  p->split_k = splits((int64_t)a->n_k_tiles * a->Hkv, (int64_t)p->a.nsub * (((int64_t)a->max_q * p->a.pg + bn - 1) / bn),
-                      (double)p->a.group * a->total_q / n / bn, 2 * krows * a->D * 4);
+                      qrows * (a->D + 1) * 4, SLOTS);
+  const int bp = bn / p->a.pg;
+  p->split_k = splits((int64_t)a->n_k_tiles * a->Hkv, (int64_t)p->a.nsub * ((a->max_q + bp - 1) / bp),
+                      (double)p->a.nsub * a->total_q / n / bp, 2 * krows * a->D * 4, p->dp == 128 ? SLOTS / 2 : SLOTS);
   return 0;
 }
 
@@ -125,7 +134,8 @@ int64_t carve(Plan* p, int backward) {
 }
 
 bool aligned(const void* p, int64_t ts, int64_t hs, int size) {
-  return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && (ts * size) % 16 == 0 && (hs * size) % 16 == 0;
+  return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && (ts * size) % 16 == 0 && (hs * size) % 16 == 0 && ts >= 0 && hs >= 0 &&
+         ts < MAX_STRIDE && hs < MAX_STRIDE;
 }
 
 int check(const Plan& p, int64_t bytes, int backward) {
