@@ -49,20 +49,24 @@ class _NormArgs(C.Structure):
         (C.c_void_p, "dx dbranch dgate dpre_w dpre_b dpost_w dpost_b workspace")])
 
 
-class _on:
-    """The tensors' device made current for the launches (nothing to do where it is already)."""
+_FN = {}
 
-    def __init__(self, device):
-        self.guard = None if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-        return torch.cuda.current_stream().cuda_stream
-
-    def __exit__(self, *e):
-        if self.guard is not None:
-            self.guard.__exit__(*e)
+def _lib_call(name, device, *args):
+    """vaesne_<name>(*args, stream) on `device`'s current stream, with `device` current; raises on a HIP
+    error as _lib.lib does.  (Looked up once, and the raw stream asked for: these calls last a few
+    microseconds on the device.)"""
+    fn = _FN.get(name)
+    if fn is None:
+        fn = _FN[name] = getattr(_lib.load(), "vaesne_" + name)
+    index = device.index
+    if index == torch._C._cuda_getDevice():
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if rc != 0:
+        raise RuntimeError(f"vaesne_{name} failed: hipError {rc}")
 
 
 def _type_of(name, *ts):
@@ -133,7 +137,7 @@ class PackedSequences:
         self._tables = {}
         self._calls = {}
         self._index = None
-        self._stream = torch.cuda.current_stream(self.device)
+        self._stream = torch._C._cuda_getCurrentRawStream(self.device.index)
 
     @classmethod
     def from_mask(cls, mask):
@@ -219,8 +223,8 @@ class PackedSequences:
 
     def _args(self, call):
         """A fresh argument struct of `call`; the tables are noted on the stream that will read them."""
-        cur = torch.cuda.current_stream(self.device)
-        if cur != self._stream:
+        if torch._C._cuda_getCurrentRawStream(self.device.index) != self._stream:
+            cur = torch.cuda.current_stream(self.device)
             for t in call[2]:
                 t.record_stream(cur)
         return _AttnArgs.from_buffer_copy(call[0])
@@ -297,8 +301,7 @@ def _attn_fwd(q, k, v, seqs, call, scale, table, lut):
     a.o, a.lse, a.workspace = o.data_ptr(), lse.data_ptr(), ws.data_ptr()
     if table is not None:
         a.table, a.lut = table.data_ptr(), lut.data_ptr()
-    with _on(q.device) as s:
-        lib.packed_attn_fwd(C.addressof(a), s)
+    _lib_call("packed_attn_fwd", q.device, C.addressof(a))
     return o, lse
 
 
@@ -334,8 +337,7 @@ class PackedAttnFn(torch.autograd.Function):
             if ctx.needs_input_grad[3]:
                 dtable = torch.empty_like(table)
                 a.dtable = dtable.data_ptr()
-        with _on(q.device) as s:
-            lib.packed_attn_bwd(C.addressof(a), s)
+        _lib_call("packed_attn_bwd", q.device, C.addressof(a))
         ng = ctx.needs_input_grad
         return dq if ng[0] else None, dk if ng[1] else None, dv if ng[2] else None, dtable, None, None, None, None
 
@@ -405,8 +407,7 @@ def _norm_fwd(a, x, branch, rows, want_stats):
     a.n = n.data_ptr()
     a.y = None if y is None else y.data_ptr()
     a.stats = None if stats is None else stats.data_ptr()
-    with _on(x.device) as s:
-        lib.gated_norm_fwd(C.addressof(a), s)
+    _lib_call("gated_norm_fwd", x.device, C.addressof(a))
     return y, n, stats
 
 
@@ -450,8 +451,7 @@ class GatedNormFn(torch.autograd.Function):
                       *[None if s is None else s.data_ptr() for s in (dx, dbr, dgate, *dp)])
         ws = _ws(lib.gated_norm_workspace(C.addressof(a)), dev)
         a.workspace = ws.data_ptr()
-        with _on(dev) as s:
-            lib.gated_norm_bwd(C.addressof(a), s)
+        _lib_call("gated_norm_bwd", dev, C.addressof(a))
         out = (dx, dbr, dp[0], dp[2], dp[1], dp[3], dgate)
         return tuple(g if n else None for g, n in zip(out, ctx.needs_input_grad)) + (None,) * 4
 
@@ -527,8 +527,7 @@ def pack8(x):
     type_ = _type_of("pack8", x)
     x = x.detach().contiguous()
     codes, exps = _codes_for(x)
-    with _on(x.device) as s:
-        lib.pack8(type_, x.data_ptr(), x.numel(), codes.data_ptr(), exps.data_ptr(), s)
+    _lib_call("pack8", x.device, type_, x.data_ptr(), x.numel(), codes.data_ptr(), exps.data_ptr())
     return Packed8(codes, exps, x.shape, x.dtype)
 
 
@@ -541,25 +540,22 @@ def unpack8(packed):
 
 def _unpack(codes, exps, shape, dtype):
     out = torch.empty(shape, dtype=dtype, device=codes.device)
-    with _on(codes.device) as s:
-        lib.unpack8(TYPES[dtype], codes.data_ptr(), exps.data_ptr(), out.numel(), out.data_ptr(), s)
+    _lib_call("unpack8", codes.device, TYPES[dtype], codes.data_ptr(), exps.data_ptr(), out.numel(), out.data_ptr())
     return out
 
 
 def _gelu8_fwd(x):
     y = torch.empty_like(x)
     codes, exps = _codes_for(x)
-    with _on(x.device) as s:
-        lib.gelu8_fwd(TYPES[x.dtype], x.data_ptr(), x.numel(), y.data_ptr(), codes.data_ptr(), exps.data_ptr(), s)
+    _lib_call("gelu8_fwd", x.device, TYPES[x.dtype], x.data_ptr(), x.numel(), y.data_ptr(), codes.data_ptr(), exps.data_ptr())
     return y, codes, exps
 
 
 def _gelu8_bwd(codes, exps, dy, again):
     dx = torch.empty_like(dy)
     y = torch.empty_like(dy) if again else None
-    with _on(dy.device) as s:
-        lib.gelu8_bwd(TYPES[dy.dtype], codes.data_ptr(), exps.data_ptr(), dy.data_ptr(), dy.numel(), dx.data_ptr(),
-                      None if y is None else y.data_ptr(), s)
+    _lib_call("gelu8_bwd", dy.device, TYPES[dy.dtype], codes.data_ptr(), exps.data_ptr(), dy.data_ptr(), dy.numel(), dx.data_ptr(),
+                      None if y is None else y.data_ptr())
     return dx, y
 
 

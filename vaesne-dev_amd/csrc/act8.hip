@@ -3,7 +3,9 @@
 // block's largest |x| is an integer maximum of bit patterns over the quad (two DPP moves), which also
 // finds infinities and NaN.  The step is a power of two, so scaling, rounding and reading back are
 // exact but for the one rounding to a whole code.  Bound by HBM: forward reads x and writes y, the
-// codes and 1/32 byte of exponents for each value.
+// codes and 1/32 byte of exponents for each value (8192 x 16384 bf16: 675 MB either way, forward 0.124 ms,
+// backward 0.143 ms, 5.4 and 4.7 TB/s; a copy of 1 GiB reaches 5.2).  16 values per thread: 0.123 and
+// 0.173 ms; one ldexp per value in place of a product with the block's step: backward 0.160 ms.
 #include "common.h"
 
 using namespace vaesne;
@@ -99,9 +101,9 @@ __device__ __forceinline__ f8 decode(const int8_t* codes, const uint8_t* exps, i
     for (int k = 0; k < 8; ++k)
       if (i + k < n) w[k >> 2] |= (uint32_t)(uint8_t)codes[i + k] << (8 * (k & 3));
   }
+  const float step = e == 255 ? __builtin_nanf("") : ldexpf(1.f, e - 133);   // (2^-132 and up: subnormal, exact)
 #pragma unroll
-  for (int k = 0; k < 8; ++k)
-    v[k] = e == 255 ? __builtin_nanf("") : ldexpf((float)(int8_t)(w[k >> 2] >> (8 * (k & 3))), e - 133);
+  for (int k = 0; k < 8; ++k) v[k] = (float)(int8_t)(w[k >> 2] >> (8 * (k & 3))) * step;
   return v;
 }
 

@@ -20,7 +20,19 @@ namespace {
 
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 
-constexpr int NT = 256;
+// threads of a workgroup: a row's, at least 256 (smaller rows share one)
+template <int P> constexpr int NT = P > 256 ? P : 256;
+template <int P> constexpr bool WHOLE = P >= 256;      // one row per workgroup
+
+// V elements of T as loaded
+template <class T, int V> struct Raw {
+  u4 r;
+  __device__ __forceinline__ void load(const T* p) { r = *reinterpret_cast<const u4*>(p); }
+};
+template <class T> struct Raw<T, 1> {
+  T r;
+  __device__ __forceinline__ void load(const T* p) { r = *p; }
+};
 
 // V elements of T as fp32; V = 1 for widths or alignments that do not allow 16-byte chunks
 template <class T, int V> struct Chunk {
@@ -35,6 +47,12 @@ template <class T, int V> struct Chunk {
 #pragma unroll
       for (int e = 0; e < V; ++e) v[e] = (float)t[e];
     }
+  }
+  __device__ __forceinline__ void take(const Raw<T, V>& x) {
+    T t[V];
+    __builtin_memcpy(t, &x.r, sizeof(t));
+#pragma unroll
+    for (int e = 0; e < V; ++e) v[e] = (float)t[e];
   }
   __device__ __forceinline__ void store(T* p) const {
     if constexpr (V == 1) {
@@ -54,7 +72,15 @@ template <class T, int V> struct Chunk {
   }
 };
 
-// sum over the P threads of a row; P = 256 goes through LDS (`buf`: 4 floats, alternating)
+// sum over a workgroup's waves' values in LDS, in order
+template <int P> __device__ __forceinline__ float lds_sum(const float* buf) {
+  float x = buf[0];
+#pragma unroll
+  for (int i = 1; i < P / 64; ++i) x += buf[i];
+  return x;
+}
+
+// sum over the P threads of a row; a whole workgroup's goes through LDS (`buf`: 8 floats, not the last call's)
 template <int P> __device__ __forceinline__ float row_sum(float x, float* buf) {
   if constexpr (P == 8) {
     x += dpp_mov<0xb1>(x);
@@ -63,10 +89,10 @@ template <int P> __device__ __forceinline__ float row_sum(float x, float* buf) {
     return x;
   } else {
     x = wave_sum(x);
-    if constexpr (P == 256) {
+    if constexpr (WHOLE<P>) {
       if ((threadIdx.x & 63) == 0) buf[threadIdx.x >> 6] = x;
       __syncthreads();
-      x = (buf[0] + buf[1]) + (buf[2] + buf[3]);
+      x = lds_sum<P>(buf);
     }
     return x;
   }
@@ -104,17 +130,17 @@ __device__ __forceinline__ void stats_of(const Chunk<T, V> (&v)[NV], int C, int 
         q = fmaf(d, d, q);
       }
   // 1 / sqrt: the root and the quotient are rounded once each
-  rstd = 1.f / sqrtf(row_sum<P>(q, red + 4) / (float)C + eps);
+  rstd = 1.f / sqrtf(row_sum<P>(q, red + 8) / (float)C + eps);
 }
 
-template <class T, int P, int V, int NV> __global__ __launch_bounds__(NT) void fwd_kernel(NArgs a) {
-  __shared__ float red[16];
-  constexpr int RPB = NT / P;
+template <class T, int P, int V, int NV> __global__ __launch_bounds__(NT<P>) void fwd_kernel(NArgs a) {
+  __shared__ float red[32];
+  constexpr int RPB = NT<P> / P;
   const vaesne_gated_norm& p = a.p;
   const int tid = threadIdx.x % P, C = p.C;
   const int64_t r = (int64_t)blockIdx.x * RPB + threadIdx.x / P;
   const bool live = r < p.rows, layer = p.kind == 1;
-  if (P == NT && !live) return;                       // (whole workgroups only)
+  if (WHOLE<P> && !live) return;                       // (whole workgroups only)
   Chunk<T, V> x[NV], f[NV];
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
@@ -146,7 +172,7 @@ template <class T, int P, int V, int NV> __global__ __launch_bounds__(NT) void f
     }
     if (p.y) x[i].store(reinterpret_cast<T*>(p.y) + r * C + c);
   }
-  stats_of<T, P, V, NV>(x, C, tid, layer, p.eps, red + 8, m2, r2);
+  stats_of<T, P, V, NV>(x, C, tid, layer, p.eps, red + 16, m2, r2);
   if (!live) return;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
@@ -174,13 +200,13 @@ __device__ __forceinline__ void norm_back(Chunk<T, V> (&d)[NV], const Chunk<T, V
       if (LAYER) s += d[i].v[e];
       q = fmaf(d[i].v[e], hat[i].v[e], q);
     }
-  if constexpr (P == NT) {
+  if constexpr (WHOLE<P>) {
     if (LAYER) s = wave_sum(s);
     q = wave_sum(q);
-    if ((threadIdx.x & 63) == 0) { red[threadIdx.x >> 6] = q; if (LAYER) red[4 + (threadIdx.x >> 6)] = s; }
+    if ((threadIdx.x & 63) == 0) { red[threadIdx.x >> 6] = q; if (LAYER) red[8 + (threadIdx.x >> 6)] = s; }
     __syncthreads();
-    q = (red[0] + red[1]) + (red[2] + red[3]);
-    if (LAYER) s = (red[4] + red[5]) + (red[6] + red[7]);
+    q = lds_sum<P>(red);
+    if (LAYER) s = lds_sum<P>(red + 8);
   } else {
     if (LAYER) s = row_sum<P>(s, red);
     q = row_sum<P>(q, red);
@@ -193,10 +219,10 @@ __device__ __forceinline__ void norm_back(Chunk<T, V> (&d)[NV], const Chunk<T, V
     for (int e = 0; e < V; ++e) d[i].v[e] = rstd * (d[i].v[e] - hat[i].v[e] * q - (LAYER ? s : 0.f));
 }
 
-template <class T, int P, int V, int NV, bool LAYER> __global__ __launch_bounds__(NT) void bwd_kernel(NArgs a) {
-  constexpr int RPB = NT / P, K = LAYER ? 5 : 3, COLS = P * V * NV;
-  __shared__ float red[16];
-  __shared__ float sums[P == NT ? 1 : 4 * COLS];
+template <class T, int P, int V, int NV, bool LAYER> __global__ __launch_bounds__(NT<P>) void bwd_kernel(NArgs a) {
+  constexpr int RPB = NT<P> / P, K = LAYER ? 5 : 3, COLS = P * V * NV;
+  __shared__ float red[32];
+  __shared__ float sums[WHOLE<P> ? 1 : 4 * COLS];
   const vaesne_gated_norm& p = a.p;
   const int tid = threadIdx.x % P, C = p.C;
   const float cs = p.residual_scale;
@@ -207,37 +233,73 @@ template <class T, int P, int V, int NV, bool LAYER> __global__ __launch_bounds_
     for (int i = 0; i < NV; ++i)
 #pragma unroll
       for (int e = 0; e < V; ++e) acc[k][i][e] = 0.f;
+  // the next turn's rows are in flight during this turn's sums (without: 309 us at 16384 x 4096 bf16
+  // with a gate per token, with: 238 us)
+  Raw<T, V> rx[NV], rf[NV], rd[NV], rG[NV], rg[NV];
+  float4 rst = make_float4(0.f, 0.f, 0.f, 0.f);
+  auto fetch = [&](int64_t r) {
+    if (r >= p.rows) return;
+    rst = *reinterpret_cast<const float4*>(p.stats + 4 * r);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = (i * P + tid) * V;
+      if (c >= C) continue;
+      rx[i].load(row_at<T>(p.x, r, p.ldx) + c);
+      if (p.branch) rf[i].load(row_at<T>(p.branch, r, p.ldbranch) + c);
+      if (p.gate_kind == 2) rg[i].load(row_at<T>(p.gate, r, p.ldgate) + c);
+      if (p.dy) rG[i].load(row_at<T>(p.dy, r, p.lddy) + c);
+      if (p.dn) rd[i].load(row_at<T>(p.dn, r, p.lddn) + c);
+    }
+  };
+  constexpr bool AHEAD = V > 1 && NV < 4;             // (single elements and 4 chunks: it spills)
+  const int64_t turn = (int64_t)gridDim.x * RPB;
+  if (AHEAD) fetch((int64_t)blockIdx.x * RPB + threadIdx.x / P);
   // every thread of a workgroup takes the same number of turns (the row sums hold barriers)
-  for (int64_t r0 = (int64_t)blockIdx.x * RPB; r0 < p.rows; r0 += (int64_t)gridDim.x * RPB) {
+  for (int64_t r0 = (int64_t)blockIdx.x * RPB; r0 < p.rows; r0 += turn) {
     const int64_t r = r0 + threadIdx.x / P;
     const bool live = r < p.rows;
-    float4 st = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (live) st = *reinterpret_cast<const float4*>(p.stats + 4 * r);
+    float4 st = rst;
+    if (!AHEAD && live) st = *reinterpret_cast<const float4*>(p.stats + 4 * r);
     Chunk<T, V> fh[NV], yh[NV], d[NV], g[NV], G[NV];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int c = (i * P + tid) * V;
       fh[i].fill(0.f); yh[i].fill(0.f); d[i].fill(0.f); g[i].fill(0.f); G[i].fill(0.f);
       if (!live || c >= C) continue;
+      if (AHEAD) {
+        yh[i].take(rx[i]);
+        if (p.branch) fh[i].take(rf[i]);
+        if (p.gate_kind == 2) g[i].take(rg[i]);
+        if (p.dy) G[i].take(rG[i]);
+        if (p.dn) d[i].take(rd[i]);
+      } else {
+        yh[i].load(row_at<T>(p.x, r, p.ldx) + c);
+        if (p.branch) fh[i].load(row_at<T>(p.branch, r, p.ldbranch) + c);
+        if (p.gate_kind == 2) g[i].load(row_at<T>(p.gate, r, p.ldgate) + c);
+        if (p.dy) G[i].load(row_at<T>(p.dy, r, p.lddy) + c);
+        if (p.dn) d[i].load(row_at<T>(p.dn, r, p.lddn) + c);
+      }
+    }
+    if (AHEAD) fetch(r + turn);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = (i * P + tid) * V;
+      if (!live || c >= C) continue;
       Chunk<T, V> w, b;
-      yh[i].load(row_at<T>(p.x, r, p.ldx) + c);
 #pragma unroll
       for (int e = 0; e < V; ++e) yh[i].v[e] *= cs;
       if (p.branch) {
-        fh[i].load(row_at<T>(p.branch, r, p.ldbranch) + c);
         w.load(row_at<T>(p.post_w, 0, 0) + c);
         b.fill(0.f);
-        g[i].fill(1.f);
         if (LAYER && p.post_b) b.load(row_at<T>(p.post_b, 0, 0) + c);
-        if (p.gate_kind) g[i].load(row_at<T>(p.gate, p.gate_kind == 2 ? r : 0, p.ldgate) + c);
+        if (p.gate_kind == 0) g[i].fill(1.f);
+        if (p.gate_kind == 1) g[i].load(row_at<T>(p.gate, 0, 0) + c);
 #pragma unroll
         for (int e = 0; e < V; ++e) {
           fh[i].v[e] = (fh[i].v[e] - st.x) * st.y;
           yh[i].v[e] = fmaf(g[i].v[e], fmaf(fh[i].v[e], w.v[e], b.v[e]), yh[i].v[e]);
         }
       }
-      if (p.dy) G[i].load(row_at<T>(p.dy, r, p.lddy) + c);
-      if (p.dn) d[i].load(row_at<T>(p.dn, r, p.lddn) + c);
       w.load(row_at<T>(p.pre_w, 0, 0) + c);
 #pragma unroll
       for (int e = 0; e < V; ++e) {
@@ -275,21 +337,21 @@ template <class T, int P, int V, int NV, bool LAYER> __global__ __launch_bounds_
       if (p.gate_kind == 2 && p.dgate) o.store(reinterpret_cast<T*>(p.dgate) + r * C + c);
     }
     if (p.branch) {
-      norm_back<T, P, V, NV, LAYER>(d, fh, st.y, C, red + 8);
+      norm_back<T, P, V, NV, LAYER>(d, fh, st.y, C, red + 16);
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
         const int c = (i * P + tid) * V;
         if (live && c < C) d[i].store(reinterpret_cast<T*>(p.dbranch) + r * C + c);
       }
-    } else if (P == NT) {
-      __syncthreads();                                // the next row's sums reuse red[0..7]
+    } else if (WHOLE<P>) {
+      __syncthreads();                                // the next row's sums reuse red[0..15]
     }
   }
   // this workgroup's column sums, rows of the same column added in a fixed order
 #pragma unroll
   for (int k = 0; k < K; ++k) {
     float* out = a.partial + ((int64_t)blockIdx.x * 5 + k) * C;
-    if constexpr (P == NT) {
+    if constexpr (WHOLE<P>) {
 #pragma unroll
       for (int i = 0; i < NV; ++i)
 #pragma unroll
@@ -312,7 +374,7 @@ template <class T, int P, int V, int NV, bool LAYER> __global__ __launch_bounds_
           if ((threadIdx.x & 63) < P) mine[(i * P + tid) * V + e] = x;
         }
       __syncthreads();
-      for (int c = threadIdx.x; c < C; c += NT) out[c] = (sums[c] + sums[COLS + c]) + (sums[2 * COLS + c] + sums[3 * COLS + c]);
+      for (int c = threadIdx.x; c < C; c += NT<P>) out[c] = (sums[c] + sums[COLS + c]) + (sums[2 * COLS + c] + sums[3 * COLS + c]);
     }
   }
 }
@@ -337,20 +399,21 @@ template <class T> __global__ __launch_bounds__(1024) void param_kernel(const fl
   }
 }
 
-// threads per row: 8 for the models' own widths, a wave up to 256 chunks, else a workgroup
+// threads per row: 8 for the models' own widths, a wave, then a workgroup; at most 16 columns each (with 32
+// the backward's sums and the rows ahead spill)
 struct Shape { int V, P, NV; };
 Shape shape_of(int C, int V) {
   const int n = (C + V - 1) / V;
   if (V > 1 && n <= 8) return {V, 8, 1};
-  if (V == 1) return n <= 256 ? Shape{1, 64, 4} : n <= 2048 ? Shape{1, 256, 8} : Shape{1, 256, 32};
+  if (V == 1) return n <= 256 ? Shape{1, 64, 4} : n <= 2048 ? Shape{1, 256, 8} : Shape{1, 512, 16};
   if (n <= 64) return {V, 64, 1};
   if (n <= 128) return {V, 64, 2};
-  if (n <= 256) return {V, 64, 4};
+  if (n <= 256) return {V, V == 4 ? 64 : 256, V == 4 ? 4 : 1};
   if (n <= 512) return {V, 256, 2};
-  return n <= 1024 ? Shape{V, 256, 4} : Shape{V, 256, 8};
+  return n <= 1024 ? Shape{V, 512, 2} : Shape{V, 512, 4};
 }
 int groups_of(const vaesne_gated_norm& a, int P) {
-  const int64_t rpb = NT / P;
+  const int64_t rpb = P > 256 ? 1 : 256 / P;
   return (int)std::max<int64_t>(1, std::min<int64_t>(512, (a.rows + rpb - 1) / rpb));
 }
 
@@ -371,15 +434,15 @@ int chunk_of(const vaesne_gated_norm& a) {
 }
 
 template <class T, int P, int V, int NV> int go(const NArgs& a, bool backward, hipStream_t s) {
-  const int64_t rpb = NT / P;
+  const int64_t rpb = NT<P> / P;
   if (!backward) {
-    hipLaunchKernelGGL((fwd_kernel<T, P, V, NV>), dim3((unsigned)((a.p.rows + rpb - 1) / rpb)), dim3(NT), 0, s, a);
+    hipLaunchKernelGGL((fwd_kernel<T, P, V, NV>), dim3((unsigned)((a.p.rows + rpb - 1) / rpb)), dim3(NT<P>), 0, s, a);
     VAESNE_CHECK_LAUNCH();
     return 0;
   }
   const int G = groups_of(a.p, P);
-  if (a.p.kind) hipLaunchKernelGGL((bwd_kernel<T, P, V, NV, true>), dim3(G), dim3(NT), 0, s, a);
-  else hipLaunchKernelGGL((bwd_kernel<T, P, V, NV, false>), dim3(G), dim3(NT), 0, s, a);
+  if (a.p.kind) hipLaunchKernelGGL((bwd_kernel<T, P, V, NV, true>), dim3(G), dim3(NT<P>), 0, s, a);
+  else hipLaunchKernelGGL((bwd_kernel<T, P, V, NV, false>), dim3(G), dim3(NT<P>), 0, s, a);
   VAESNE_CHECK_LAUNCH();
   Outs o = {{a.p.dpre_w, a.p.dpost_w, a.p.gate_kind == 1 ? a.p.dgate : nullptr, a.p.kind ? a.p.dpre_b : nullptr,
              a.p.kind ? a.p.dpost_b : nullptr}};
@@ -393,9 +456,10 @@ template <class T> int run(const vaesne_gated_norm& p, bool backward, hipStream_
   const NArgs a{p, reinterpret_cast<float*>(p.workspace)};
   const Shape q = shape_of(p.C, chunk_of(p));
 #define VAESNE_GN(PV, VV, NVV) if (q.P == PV && q.V == VV && q.NV == NVV) return go<T, PV, VV, NVV>(a, backward, s);
-  VAESNE_GN(8, W, 1) VAESNE_GN(64, W, 1) VAESNE_GN(64, W, 2) VAESNE_GN(64, W, 4) VAESNE_GN(256, W, 2) VAESNE_GN(256, W, 4)
-  if constexpr (W == 4) { VAESNE_GN(256, W, 8) }
-  VAESNE_GN(64, 1, 4) VAESNE_GN(256, 1, 8) VAESNE_GN(256, 1, 32)
+  VAESNE_GN(8, W, 1) VAESNE_GN(64, W, 1) VAESNE_GN(64, W, 2) VAESNE_GN(256, W, 2) VAESNE_GN(512, W, 2)
+  if constexpr (W == 4) { VAESNE_GN(64, W, 4) VAESNE_GN(512, W, 4) }
+  else { VAESNE_GN(256, W, 1) }
+  VAESNE_GN(64, 1, 4) VAESNE_GN(256, 1, 8) VAESNE_GN(512, 1, 16)
 #undef VAESNE_GN
   return (int)hipErrorInvalidValue;
 }
@@ -410,7 +474,7 @@ int dispatch(const vaesne_gated_norm* a, bool backward, void* stream) {
 VAESNE_API int64_t vaesne_gated_norm_workspace(const vaesne_gated_norm* a) {
   if (bad(a)) return -1;
   // the most workgroups any chunk width gives: 8 threads per row never give more than a whole one
-  return (int64_t)groups_of(*a, NT) * 5 * a->C * 4;
+  return (int64_t)groups_of(*a, 256) * 5 * a->C * 4;
 }
 
 VAESNE_API int vaesne_gated_norm_fwd(const vaesne_gated_norm* a, void* stream) {

@@ -52,6 +52,7 @@ constexpr float INF = __builtin_inff();
 struct Args {
   vaesne_packed_attn p;
   int pg, nsub, group;         // heads per tile, tiles per key head's group, query heads per key head
+  int pk_log, nsubk;           // dK / dV: log2(heads per row tile), tiles per group
   uint32_t pgm;                // ceil(2^32 / pg), 0 for pg = 1
   int nsplit;
   float c;                     // scale * log2(e)
@@ -109,31 +110,49 @@ template <class T, int DP> struct Tile {
   }
   static __device__ __forceinline__ int at(int r, int c) { return r * RB + ((c ^ swz(r)) << 4); }
 
-  // lane's fragment of row r: columns KC k + EPC h ..
-  static __device__ __forceinline__ typename Ty<T>::Frag row(const char* s, int r, int k, int h) {
-    return *reinterpret_cast<const typename Ty<T>::Frag*>(s + at(r, 2 * k + h));
+  // A lane's LDS offsets.  swz is a combination of xors of row bits, so a fragment's address is one
+  // of these, xor a constant, plus a constant (a multiple of 16 rows, the tile): nothing but the
+  // offsets stays in registers.  (Addresses kept for every fragment took 24 registers of each wave.)
+  struct Lane {
+    uint32_t r, c[2];
+    __device__ __forceinline__ Lane(int lane) {
+      const int h = lane >> 5, i = lane & 15;
+      r = at(lane & 31, h);
+      if constexpr (sizeof(T) == 2) {
+        const int ch = (2 * ((lane >> 4) & 1) + ((i & 3) >> 1)) & (CPR - 1);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) c[j] = at(8 * j + 4 * h + (i >> 2), ch) + 8 * (i & 1);
+      } else {
+        c[0] = at(4 * h, ((lane & 31) >> 2) & (CPR - 1)) + 4 * (lane & 3);
+        c[1] = 0;
+      }
+    }
+    // not known to be the same from one tile to the next: the xors are taken again, not kept
+    __device__ __forceinline__ void renew() { asm volatile("" : "+v"(r), "+v"(c[0]), "+v"(c[1])); }
+  };
+  // fragment of row r0 + lane % 32 (r0: a multiple of 32): columns KC k + EPC h ..
+  static __device__ __forceinline__ typename Ty<T>::Frag row(const char* s, const Lane& l, int r0, int k) {
+    return *reinterpret_cast<const typename Ty<T>::Frag*>(s + r0 * RB + (l.r ^ (k << 5)));
   }
   // transposed fragment: column 32 dt + lane % 32 of rows r0 + (block t's slots)
-  static __device__ __forceinline__ typename Ty<T>::Frag col(const char* s, int r0, int t, int dt, int lane) {
-    const int h = lane >> 5;
+  static __device__ __forceinline__ typename Ty<T>::Frag col(const char* s, const Lane& l, int r0, int t, int dt) {
     if constexpr (sizeof(T) == 2) {
-      const int i = lane & 15, c = (4 * dt + 2 * ((lane >> 4) & 1) + ((i & 3) >> 1)) & (CPR - 1);
       u4 o;
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        const int r = r0 + KC * t + 8 * j + 4 * h + (i >> 2);
         const s4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-            (__attribute__((address_space(3))) s4*)(s + at(r, c) + 8 * (i & 1)));
+            (__attribute__((address_space(3))) s4*)(s + (r0 + KC * t) * RB + (l.c[j] ^ (CPR > 4 ? dt << 6 : 0))));
         const uint2 y = __builtin_bit_cast(uint2, x);
         o[2 * j] = y.x; o[2 * j + 1] = y.y;
       }
       return __builtin_bit_cast(typename Ty<T>::Frag, o);
     } else {
-      const int d = 32 * dt + (lane & 31);
       typename Ty<T>::Frag o;
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        o[j] = *reinterpret_cast<const float*>(s + at(r0 + KC * t + 4 * h + j, (d >> 2) & (CPR - 1)) + 4 * (d & 3));
+      for (int j = 0; j < 4; ++j) {
+        const int f = (CPR >= 16 ? j << 2 : CPR == 8 ? (j >> 1) << 2 : 0) ^ (2 * (t & 1)) ^ (CPR > 8 ? 8 * dt : 0);
+        o[j] = *reinterpret_cast<const float*>(s + (r0 + KC * t + j) * RB + (l.c[0] ^ (f << 4)));
+      }
       return o;
     }
   }
@@ -143,25 +162,22 @@ template <class T, int DP> struct Tile {
 // offsets from the tile's first row never change, so a tile costs one buffer descriptor (scalar) and
 // no address arithmetic; an absent chunk's offset lies outside the descriptor and reads as zero.
 // (With 64-bit addresses computed for every chunk the forward issued 10 vector instructions per
-// score, with this 6.)  EVEN: rows lie at one stride, and a thread's chunks differ by a scalar step.
+// score, with this 7.)  A thread's chunks lie RS rows apart, a scalar step.
 constexpr uint32_t NO_ROW = 0x80000000u;
-template <class T, int DP, int ROWS, int NT, bool EVEN> struct Stage {
+template <class T, int DP, int ROWS, int NT> struct Stage {
   using L = Tile<T, DP>;
+  static_assert(NT % L::CPR == 0 && (ROWS * L::CPR < NT || ROWS * L::CPR % NT == 0), "whole rows per turn");
   static constexpr int CH = ROWS * L::CPR;
   static constexpr int NI = (CH + NT - 1) / NT;
   static constexpr int RS = NT / L::CPR;              // rows between a thread's chunks
   u4 v[NI];
-  uint32_t off[EVEN ? 1 : NI];
+  uint32_t off;
   int step;
-  // bytes(r): row r's distance from the tile's first row, NO_ROW for a row no tile has
+  // bytes(r): row r's distance from the tile's first row
   template <class Bytes> __device__ __forceinline__ void init(int D, Bytes bytes) {
-#pragma unroll
-    for (int i = 0; i < (EVEN ? 1 : NI); ++i) {
-      const int id = threadIdx.x + i * NT, r = id / L::CPR, c = id % L::CPR;
-      const uint32_t b = (CH % NT != 0 && id >= CH) || c * L::EPC >= D ? NO_ROW : bytes(r);
-      off[i] = b == NO_ROW ? b : b + 16 * c;
-    }
-    step = EVEN ? (int)bytes(RS) : 0;
+    const int r = threadIdx.x / L::CPR, c = threadIdx.x % L::CPR;
+    off = (CH < NT && (int)threadIdx.x >= CH) || c * L::EPC >= D ? NO_ROW : bytes(r) + 16 * c;
+    step = (int)bytes(RS);
   }
   // rows 0 .. left - 1 from `first` (uniform over the workgroup)
   __device__ __forceinline__ void load(const T* first, int left) {
@@ -170,13 +186,13 @@ template <class T, int DP, int ROWS, int NT, bool EVEN> struct Stage {
     // (one load for whole and partial tiles: two alternatives would be merged behind a wait)
 #pragma unroll
     for (int i = 0; i < NI; ++i)
-      v[i] = __builtin_amdgcn_raw_buffer_load_b128(rsrc, r < left - i * RS ? off[EVEN ? 0 : i] : NO_ROW, i * step, 0);
+      v[i] = __builtin_amdgcn_raw_buffer_load_b128(rsrc, r < left - i * RS ? off : NO_ROW, i * step, 0);
   }
   __device__ __forceinline__ void store(char* s) const {
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
       const int id = threadIdx.x + i * NT;
-      if (CH % NT != 0 && id >= CH) continue;
+      if (CH < NT && id >= CH) continue;
       *reinterpret_cast<u4*>(s + L::at(id / L::CPR, id % L::CPR)) = v[i];
     }
   }
@@ -300,7 +316,13 @@ template <class T, int DP> constexpr int key_tile() { return sizeof(T) == 2 ? 64
 template <class T, int DP, bool BIAS, int NW, bool DQ> constexpr int occ() {
   return DP == 128 && (sizeof(T) == 4 || NW == 2 || (DQ && BIAS)) ? 1 : 2;
 }
-template <class T, int DP> constexpr int occ_kv() { return DP == 128 || (sizeof(T) == 4 && DP == 64) ? 1 : 2; }
+// dK / dV at head_dim 128 hold 128 registers of sums: V goes to LDS and the row tile is 32, so that two
+// waves per SIMD fit (causal training step of 10 k tokens, 16 heads over 4: V in registers at one
+// wave 0.59 ms, at two, spilling, 1.50 ms; so 0.53 ms)
+template <class T, int DP> constexpr bool v_in_lds() { return sizeof(T) == 2 && DP == 128; }
+template <class T, int DP, int NW> constexpr int occ_kv() { return (sizeof(T) == 4 && DP >= 64) || (NW == 2 && DP == 128) ? 1 : 2; }
+// query rows of a tile in dK / dV
+template <class T, int DP> constexpr int row_tile() { return v_in_lds<T, DP>() ? 32 : key_tile<T, DP>(); }
 
 template <class T, int DP, bool BIAS, int NW>
 __global__ __launch_bounds__(NW * 64, (occ<T, DP, BIAS, NW, false>())) void fwd_kernel(Args a) {
@@ -336,7 +358,7 @@ __global__ __launch_bounds__(NW * 64, (occ<T, DP, BIAS, NW, false>())) void fwd_
 
   const T* kb = reinterpret_cast<const T*>(a.p.k) + t.k0 * a.p.k_ts + t.kvh * a.p.k_hs;
   const T* vb = reinterpret_cast<const T*>(a.p.v) + t.k0 * a.p.v_ts + t.kvh * a.p.v_hs;
-  Stage<T, DP, BN, NT, true> ks, vs;
+  Stage<T, DP, BN, NT> ks, vs;
   ks.init(D, [&](int r) { return (uint32_t)r * (uint32_t)(a.p.k_ts * sizeof(T)); });
   vs.init(D, [&](int r) { return (uint32_t)r * (uint32_t)(a.p.v_ts * sizeof(T)); });
   auto fetch = [&](int j) {
@@ -350,7 +372,9 @@ __global__ __launch_bounds__(NW * 64, (occ<T, DP, BIAS, NW, false>())) void fwd_
   }
   loads_done();
   __syncthreads();
+  typename L::Lane at(lane);
   auto step = [&](int j, auto buf) {
+    at.renew();
     const char* K = smem + buf.value * 2 * TILE;
     const char* V = K + TILE;
     if (j + 1 < t1) fetch(j + 1);
@@ -361,7 +385,7 @@ __global__ __launch_bounds__(NW * 64, (occ<T, DP, BIAS, NW, false>())) void fwd_
       for (int n = 0; n < NB; ++n) {
         s[n] = f16v{};
 #pragma unroll
-        for (int k = 0; k < L::NCH; ++k) s[n] = mma(L::row(K, 32 * n + (lane & 31), k, h), qf[k], s[n]);
+        for (int k = 0; k < L::NCH; ++k) s[n] = mma(L::row(K, at, 32 * n, k), qf[k], s[n]);
       }
       feed<NB * L::NCH, 1, 4>();
       // scores to the units of the running maximum: raw without a bias, log2 with one
@@ -408,7 +432,7 @@ __global__ __launch_bounds__(NW * 64, (occ<T, DP, BIAS, NW, false>())) void fwd_
         for (int b = 0; b < L::TB; ++b) {
           const auto pf = take<T>(s[n], b);
 #pragma unroll
-          for (int dt = 0; dt < L::DT; ++dt) o[dt] = mma(L::col(V, 32 * n, b, dt, lane), pf, o[dt]);
+          for (int dt = 0; dt < L::DT; ++dt) o[dt] = mma(L::col(V, at, 32 * n, b, dt), pf, o[dt]);
         }
       feed<NB * L::TB * L::DT, L::CR, 3>();
     }
@@ -443,7 +467,11 @@ __global__ __launch_bounds__(NW * 64, (occ<T, DP, BIAS, NW, false>())) void fwd_
 // workgroup, 32 lanes of 4 columns each.
 template <class T, bool WEIGHTED>
 __global__ __launch_bounds__(256) void join_kernel(const float* part, const float* part_lse, int n, int64_t rows,
-                                                   int D, T* out, float* lse) {
+                                                   int D, T* out, T* out2, float* lse) {
+  if (blockIdx.y == 1) {                               // (the second tensor's parts follow the first's)
+    part += (int64_t)n * rows * D;
+    out = out2;
+  }
   const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
   const int d = (threadIdx.x & 31) * 4;
   if (row >= rows) return;
@@ -553,7 +581,7 @@ __global__ __launch_bounds__(NW * 64, (occ<T, DP, BIAS, NW, true>())) void dq_ke
 
   const T* kb = reinterpret_cast<const T*>(a.p.k) + t.k0 * a.p.k_ts + t.kvh * a.p.k_hs;
   const T* vb = reinterpret_cast<const T*>(a.p.v) + t.k0 * a.p.v_ts + t.kvh * a.p.v_hs;
-  Stage<T, DP, BN, NT, true> ks, vs;
+  Stage<T, DP, BN, NT> ks, vs;
   ks.init(D, [&](int r) { return (uint32_t)r * (uint32_t)(a.p.k_ts * sizeof(T)); });
   vs.init(D, [&](int r) { return (uint32_t)r * (uint32_t)(a.p.v_ts * sizeof(T)); });
   auto fetch = [&](int j) {
@@ -567,7 +595,9 @@ __global__ __launch_bounds__(NW * 64, (occ<T, DP, BIAS, NW, true>())) void dq_ke
   }
   loads_done();
   __syncthreads();
+  typename L::Lane at(lane);
   auto step = [&](int j, auto buf) {
+    at.renew();
     const char* K = smem + buf.value * 2 * TILE;
     const char* V = K + TILE;
     if (j + 1 < t1) fetch(j + 1);
@@ -577,9 +607,9 @@ __global__ __launch_bounds__(NW * 64, (occ<T, DP, BIAS, NW, true>())) void dq_ke
       if (base < wmax) {
         f16v s = f16v{}, g = f16v{};
 #pragma unroll
-        for (int k = 0; k < L::NCH; ++k) s = mma(L::row(K, 32 * n + (lane & 31), k, h), qf[k], s);
+        for (int k = 0; k < L::NCH; ++k) s = mma(L::row(K, at, 32 * n, k), qf[k], s);
 #pragma unroll
-        for (int k = 0; k < L::NCH; ++k) g = mma(L::row(V, 32 * n + (lane & 31), k, h), gf[k], g);
+        for (int k = 0; k < L::NCH; ++k) g = mma(L::row(V, at, 32 * n, k), gf[k], g);
         feed<2 * L::NCH, 1, 4>();
         const float c = BIAS ? 1.f : a.c;
         const int rel0 = base - qabs;
@@ -621,7 +651,7 @@ __global__ __launch_bounds__(NW * 64, (occ<T, DP, BIAS, NW, true>())) void dq_ke
         for (int b = 0; b < L::TB; ++b) {
           const auto sf = take<T>(s, b);
 #pragma unroll
-          for (int dt = 0; dt < L::DT; ++dt) o[dt] = mma(L::col(K, 32 * n, b, dt, lane), sf, o[dt]);
+          for (int dt = 0; dt < L::DT; ++dt) o[dt] = mma(L::col(K, at, 32 * n, b, dt), sf, o[dt]);
         }
         feed<L::TB * L::DT, L::CR, 3>();
       }
@@ -685,13 +715,14 @@ __global__ __launch_bounds__(1024) void hist_bucket_kernel(const float* rel, con
 // backward: dK, dV
 // -------------------------------------------------------------------------------------------
 template <class T, int DP, bool BIAS, int NW>
-__global__ __launch_bounds__(NW * 64, (occ_kv<T, DP>())) void dkv_kernel(Args a) {
+__global__ __launch_bounds__(NW * 64, (occ_kv<T, DP, NW>())) void dkv_kernel(Args a) {
   using L = Tile<T, DP>;
-  constexpr int NT = NW * 64, BQ = key_tile<T, DP>(), NB = BQ / 32, TILE = BQ * L::RB;
-  constexpr bool HALF = __is_same(T, _Float16);
+  constexpr int NT = NW * 64, BQ = row_tile<T, DP>(), NB = BQ / 32, TILE = BQ * L::RB;
+  constexpr bool VL = v_in_lds<T, DP>(), HALF = __is_same(T, _Float16);
   extern __shared__ __attribute__((aligned(16))) char smem[];
   float* stat = reinterpret_cast<float*>(smem + 4 * TILE);     // [2][lse BQ | delta BQ]
   float* lut = stat + 4 * BQ;
+  char* vt = smem + 4 * TILE + 16 * BQ + (BIAS ? (span_of(a.p.max_distance) * 4 + 15) / 16 * 16 : 0);   // this tile's V (VL)
   const int kvh = blockIdx.x % a.p.Hkv, tile = blockIdx.x / a.p.Hkv, D = a.p.D, R = a.p.max_distance;
   const int seq = uni(a.p.k_tiles[2 * tile]), key0 = uni(a.p.k_tiles[2 * tile + 1]);
   const int64_t q0 = uni(a.p.cu_q[seq]), k0 = uni(a.p.cu_k[seq]);
@@ -699,9 +730,17 @@ __global__ __launch_bounds__(NW * 64, (occ_kv<T, DP>())) void dkv_kernel(Args a)
   const int lane = threadIdx.x & 63, w = uni(threadIdx.x >> 6), h = lane >> 5;
   const int key = key0 + w * 32 + (lane & 31);
   const bool valid = key < nk;
-  typename Ty<T>::Frag kf[L::NCH], vf[L::NCH];
+  typename Ty<T>::Frag kf[L::NCH], vf[VL ? 1 : L::NCH];
   load_frags<T, DP>(kf, valid ? reinterpret_cast<const T*>(a.p.k) + (k0 + key) * a.p.k_ts + kvh * a.p.k_hs : nullptr, D, h);
-  load_frags<T, DP>(vf, valid ? reinterpret_cast<const T*>(a.p.v) + (k0 + key) * a.p.v_ts + kvh * a.p.v_hs : nullptr, D, h);
+  const T* vp = reinterpret_cast<const T*>(a.p.v) + (k0 + key) * a.p.v_ts + kvh * a.p.v_hs;
+  if constexpr (VL) {
+    typename Ty<T>::Frag f[L::NCH];                            // each wave writes and reads its own 32 rows
+    load_frags<T, DP>(f, valid ? vp : nullptr, D, h);
+#pragma unroll
+    for (int k = 0; k < L::NCH; ++k) *reinterpret_cast<typename Ty<T>::Frag*>(vt + L::at(w * 32 + (lane & 31), 2 * k + h)) = f[k];
+  } else {
+    load_frags<T, DP>(vf, valid ? vp : nullptr, D, h);
+  }
   f16v dk[L::DT], dv[L::DT];
 #pragma unroll
   for (int i = 0; i < L::DT; ++i) dk[i] = dv[i] = f16v{};
@@ -709,33 +748,31 @@ __global__ __launch_bounds__(NW * 64, (occ_kv<T, DP>())) void dkv_kernel(Args a)
   if (HALF) up = 8.f * pow2_of(a.domax[kvh]);
   const float down = 1.f / up;
 
-  // rows (position * PG + head) that see any of the tile's keys, tile by tile, one head group after
-  // the other: it = sub * ntq + row tile.  A row tile holds whole positions: BP of them, BP PG rows.
-  const int bp = BQ / a.pg, br = bp * a.pg, nrows = nq * a.pg;
+  // rows (position * PK + head) that see any of the tile's keys, tile by tile, one head group after
+  // the other: it = sub * ntq + row tile.  PK, the heads that share a row tile, is a power of two, so a
+  // row tile holds whole positions and a thread's chunks lie whole positions apart.
+  const int lg = a.pk_log, pk = 1 << lg, bp = BQ >> lg, nrows = nq << lg;
   const int first = a.p.causal ? min(max(key0 - off, 0), nq) / bp : 0;
-  const int ntq = max((nq + bp - 1) / bp - first, 0), total = a.nsub * ntq;
+  const int ntq = max((nq + bp - 1) / bp - first, 0), total = a.nsubk * ntq;
   const int per = (total + a.nsplit - 1) / a.nsplit, t0 = blockIdx.y * per, t1 = min(total, t0 + per);
   // the first row that sees this lane's key / the wave's first and last key
-  const int see = a.p.causal ? (key - off) * a.pg : 0;
-  const int wfirst = a.p.causal ? (key0 + w * 32 - off) * a.pg : 0;
-  const int wlast = a.p.causal ? (key0 + w * 32 + 31 - off) * a.pg : 0;
+  const int see = a.p.causal ? (key - off) * pk : 0;
+  const int wfirst = a.p.causal ? (key0 + w * 32 - off) * pk : 0;
+  const int wlast = a.p.causal ? (key0 + w * 32 + 31 - off) * pk : 0;
   const bool active = key0 + w * 32 < nk;
 
-  Stage<T, DP, BQ, NT, false> qs, gs;
+  Stage<T, DP, BQ, NT> qs, gs;
   float st_l, st_d;
   bool st_in;
   auto bytes = [&](int64_t ts, int64_t hs) {
-    return [=](int r) {
-      const int pos = div_pg(a, r);
-      return r >= br ? NO_ROW : (uint32_t)((pos * ts + (r - pos * a.pg) * hs) * (int)sizeof(T));
-    };
+    return [=](int r) { return (uint32_t)(((r >> lg) * ts + (r & (pk - 1)) * hs) * (int)sizeof(T)); };
   };
   qs.init(D, bytes(a.p.q_ts, a.p.q_hs));
   gs.init(D, bytes(a.p.do_ts, a.p.do_hs));
-  const int spos = div_pg(a, threadIdx.x), sofs = spos * a.p.Hq + (int)threadIdx.x - spos * a.pg;
+  const int sofs = ((int)threadIdx.x >> lg) * a.p.Hq + ((int)threadIdx.x & (pk - 1));
   auto fetch = [&](int it) {
-    const int sub = it / ntq, pos = (first + it - sub * ntq) * bp, head0 = kvh * a.group + sub * a.pg;
-    const int left = min(nrows - pos * a.pg, br);
+    const int sub = it / ntq, pos = (first + it - sub * ntq) * bp, head0 = kvh * a.group + (sub << lg);
+    const int left = min(nrows - (pos << lg), BQ);
     qs.load(reinterpret_cast<const T*>(a.p.q) + (q0 + pos) * a.p.q_ts + head0 * a.p.q_hs, left);
     gs.load(reinterpret_cast<const T*>(a.p.dout) + (q0 + pos) * a.p.do_ts + head0 * a.p.do_hs, left);
     const int64_t rid = (q0 + pos) * a.p.Hq + head0;
@@ -759,16 +796,18 @@ __global__ __launch_bounds__(NW * 64, (occ_kv<T, DP>())) void dkv_kernel(Args a)
   }
   loads_done();
   __syncthreads();
+  typename L::Lane at(lane);
   auto step = [&](int it, auto buf) {
+    at.renew();
     constexpr int b = buf.value;
     const char* Q = smem + b * 2 * TILE;
     const char* G = Q + TILE;
     const float* lse = stat + b * 2 * BQ;
     const float* dl = lse + BQ;
-    const int sub = it / ntq, rb = (first + it - sub * ntq) * br;
+    const int sub = it / ntq, rb = (first + it - sub * ntq) * BQ;
     if (BIAS && sub != sub_now) {                              // the next head's biases
       __syncthreads();
-      load_bias<T, NT>(a, lut, kvh * a.group + sub * a.pg);
+      load_bias<T, NT>(a, lut, kvh * a.group + (sub << lg));
       __syncthreads();
       sub_now = sub;
     }
@@ -778,13 +817,10 @@ __global__ __launch_bounds__(NW * 64, (occ_kv<T, DP>())) void dkv_kernel(Args a)
 #pragma unroll
       for (int n = 0; n < NB; ++n) {
         s[n] = f16v{};
-        g[n] = f16v{};
 #pragma unroll
-        for (int k = 0; k < L::NCH; ++k) s[n] = mma(L::row(Q, 32 * n + (lane & 31), k, h), kf[k], s[n]);
-#pragma unroll
-        for (int k = 0; k < L::NCH; ++k) g[n] = mma(L::row(G, 32 * n + (lane & 31), k, h), vf[k], g[n]);
+        for (int k = 0; k < L::NCH; ++k) s[n] = mma(L::row(Q, at, 32 * n, k), kf[k], s[n]);
       }
-      feed<2 * NB * L::NCH, 1, 4>();
+      feed<NB * L::NCH, 1, 3>();
       const float c = BIAS ? 1.f : a.c;
 #pragma unroll
       for (int n = 0; n < NB; ++n) {
@@ -807,9 +843,18 @@ __global__ __launch_bounds__(NW * 64, (occ_kv<T, DP>())) void dkv_kernel(Args a)
         for (int t = 0; t < L::TB; ++t) {
           const auto pf = take<T>(s[n], t);
 #pragma unroll
-          for (int dt = 0; dt < L::DT; ++dt) dv[dt] = mma(L::col(G, 32 * n, t, dt, lane), pf, dv[dt]);
+          for (int dt = 0; dt < L::DT; ++dt) dv[dt] = mma(L::col(G, at, 32 * n, t, dt), pf, dv[dt]);
         }
         feed<L::DT * L::TB, L::CR, 3>();
+        __builtin_amdgcn_sched_barrier(0);                     // (merged with the next stage it spills)
+        g[n] = f16v{};
+#pragma unroll
+        for (int k = 0; k < L::NCH; ++k) {
+          if constexpr (VL) g[n] = mma(L::row(G, at, 32 * n, k), L::row(vt, at, w * 32, k), g[n]);
+          else g[n] = mma(L::row(G, at, 32 * n, k), vf[k], g[n]);
+        }
+        feed<L::NCH, VL ? 2 : 1, VL ? 2 : 3>();
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
           const f4 x = *reinterpret_cast<const f4*>(dl + 32 * n + 8 * q + 4 * h);
@@ -820,7 +865,7 @@ __global__ __launch_bounds__(NW * 64, (occ_kv<T, DP>())) void dkv_kernel(Args a)
         for (int t = 0; t < L::TB; ++t) {
           const auto sf = take<T>(s[n], t);
 #pragma unroll
-          for (int dt = 0; dt < L::DT; ++dt) dk[dt] = mma(L::col(Q, 32 * n, t, dt, lane), sf, dk[dt]);
+          for (int dt = 0; dt < L::DT; ++dt) dk[dt] = mma(L::col(Q, at, 32 * n, t, dt), sf, dk[dt]);
         }
         feed<L::DT * L::TB, L::CR, 3>();
       }
@@ -873,7 +918,7 @@ template <class T, int DP, bool BIAS> int fwd_dp(const Plan& p, hipStream_t s) {
   if (rc || a.nsplit == 1) return rc;
   const int64_t rows = a.p.total_q * a.p.Hq;
   hipLaunchKernelGGL((join_kernel<T, true>), dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, s, a.part, a.part_lse, a.nsplit,
-                     rows, a.p.D, reinterpret_cast<T*>(a.p.o), a.p.lse);
+                     rows, a.p.D, reinterpret_cast<T*>(a.p.o), nullptr, a.p.lse);
   VAESNE_CHECK_LAUNCH();
   return 0;
 }
@@ -898,7 +943,7 @@ template <class T, int DP, bool BIAS> int bwd_dp(const Plan& p, hipStream_t s) {
     if (a.nsplit > 1) {
       const int64_t rows = a.p.total_q * a.p.Hq;
       hipLaunchKernelGGL((join_kernel<T, false>), dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, s, a.part, nullptr,
-                         a.nsplit, rows, a.p.D, reinterpret_cast<T*>(a.p.dq), nullptr);
+                         a.nsplit, rows, a.p.D, reinterpret_cast<T*>(a.p.dq), nullptr, nullptr);
       VAESNE_CHECK_LAUNCH();
     }
   }
@@ -913,18 +958,17 @@ template <class T, int DP, bool BIAS> int bwd_dp(const Plan& p, hipStream_t s) {
   }
   if (a.p.n_k_tiles == 0) return 0;
   a.nsplit = p.split_k;
-  const size_t lds = 4 * BN * RB + 16 * BN + (BIAS ? span_of(a.p.max_distance) * 4 : 0);
+  constexpr int BQ = row_tile<T, DP>();
+  const size_t lds = 4 * BQ * RB + 16 * BQ + (BIAS ? (span_of(a.p.max_distance) * 4 + 15) / 16 * 16 : 0) +
+                     (v_in_lds<T, DP>() ? p.nwk * 32 * RB : 0);
   const int wgs = a.p.n_k_tiles * a.p.Hkv;
   const int rc = p.nwk == 2 ? launch<T>(dkv_kernel<T, DP, BIAS, 2>, dim3(wgs, a.nsplit), 128, lds, a, s)
                             : launch<T>(dkv_kernel<T, DP, BIAS, 4>, dim3(wgs, a.nsplit), 256, lds, a, s);
   if (rc || a.nsplit == 1) return rc;
   const int64_t rows = a.p.total_k * a.p.Hkv;
-  for (int i = 0; i < 2; ++i) {
-    hipLaunchKernelGGL((join_kernel<T, false>), dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, s,
-                       a.part + (int64_t)i * a.nsplit * rows * a.p.D, nullptr, a.nsplit, rows, a.p.D,
-                       reinterpret_cast<T*>(i ? a.p.dv : a.p.dk), nullptr);
-    VAESNE_CHECK_LAUNCH();
-  }
+  hipLaunchKernelGGL((join_kernel<T, false>), dim3((unsigned)((rows + 7) / 8), 2), dim3(256), 0, s, a.part, nullptr, a.nsplit,
+                     rows, a.p.D, reinterpret_cast<T*>(a.p.dk), reinterpret_cast<T*>(a.p.dv), nullptr);
+  VAESNE_CHECK_LAUNCH();
   return 0;
 }
 

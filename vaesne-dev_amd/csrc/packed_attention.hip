@@ -53,15 +53,17 @@ constexpr int64_t MAX_ROWS = 1 << 25; // rows of one sequence: 32-bit row arithm
 // forward, two 58 + 17 us; dK / dV of the bf16 training step: one part 873 us, two 680 + 22 us.)
 int splits(int64_t wgs, int64_t longest, double mean, int64_t part_bytes, int slots) {
   const double over = 6, join = 8;
-  const int64_t most = std::min<int64_t>(std::min<int64_t>(MAX_SPLIT, longest / 4), MAX_PART / std::max<int64_t>(part_bytes, 1));
-  int best = 1;
-  double least = 0;
-  for (int n = 1; n <= std::max<int64_t>(most, 1); ++n) {
+  const int64_t most = std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(MAX_SPLIT, longest / 4),
+                                                              MAX_PART / std::max<int64_t>(part_bytes, 1)));
+  auto end = [&](int64_t n) {
     const double own = (double)((longest + n - 1) / n) + over;
-    const double end = std::max(wgs * (mean + n * over) / slots + 0.5 * own, own) + (n > 1 ? join : 0);
-    if (n == 1 || end < least) { best = n; least = end; }
-  }
-  return best;
+    return std::max(wgs * (mean + n * over) / slots + 0.5 * own, own) + (n > 1 ? join : 0);
+  };
+  double least = end(1);
+  for (int64_t n = 2; n <= most; ++n) least = std::min(least, end(n));
+  for (int64_t n = 1; n < most; ++n)
+    if (end(n) <= 1.05 * least) return (int)n;         // the fewest parts that come within a twentieth
+  return (int)most;
 }
 
 int64_t up16(int64_t n) { return (n + 15) & ~(int64_t)15; }
@@ -83,6 +85,15 @@ int heads_per_tile(const vaesne_packed_attn* a) {
   return 1;
 }
 
+// the same in dK / dV: a power of two, and no more than the rows between a thread's chunks
+int log_heads_per_row_tile(const vaesne_packed_attn* a, int dp, int waves) {
+  if (a->table) return 0;
+  const int g = a->Hq / a->Hkv, rows = waves * 64 / (dp * (a->type == 0 ? 4 : 2) / 16);
+  int l = 0;
+  while (l < 5 && g % (2 << l) == 0 && (2 << l) <= rows) ++l;
+  return l;
+}
+
 int waves_for(int64_t rows) { return rows <= 64 ? 2 : 4; }
 
 int make_plan(const vaesne_packed_attn* a, Plan* p) {
@@ -98,14 +109,16 @@ int make_plan(const vaesne_packed_attn* a, Plan* p) {
   p->dp = a->D <= 16 ? 16 : a->D <= 32 ? 32 : a->D <= 64 ? 64 : 128;
   p->nwq = waves_for((int64_t)a->max_q * p->a.pg);
   p->nwk = waves_for(a->max_k);
+  p->a.pk_log = log_heads_per_row_tile(a, p->dp, p->nwk);
+  p->a.nsubk = p->a.group >> p->a.pk_log;
   const int bn = a->type == 0 ? 32 : 64;
   const int64_t qrows = a->total_q * a->Hq, krows = a->total_k * a->Hkv;
   const double n = std::max(a->nseq, 1);
   p->split_q = splits((int64_t)a->n_q_tiles * a->Hkv * p->a.nsub, (a->max_k + bn - 1) / bn, a->total_k / n / bn,
                       qrows * (a->D + 1) * 4, SLOTS);
-  const int bp = bn / p->a.pg;
-  p->split_k = splits((int64_t)a->n_k_tiles * a->Hkv, (int64_t)p->a.nsub * ((a->max_q + bp - 1) / bp),
-                      (double)p->a.nsub * a->total_q / n / bp, 2 * krows * a->D * 4, p->dp == 128 ? SLOTS / 2 : SLOTS);
+  const int bp = (a->type != 0 && p->dp == 128 ? 32 : bn) >> p->a.pk_log;   // row_tile()
+  p->split_k = splits((int64_t)a->n_k_tiles * a->Hkv, (int64_t)p->a.nsubk * ((a->max_q + bp - 1) / bp),
+                      (double)p->a.nsubk * a->total_q / n / bp, 2 * krows * a->D * 4, SLOTS);
   return 0;
 }
 
