@@ -103,6 +103,22 @@ def _lengths(lengths, name):
     return out
 
 
+def tile_table(nq, nk, side, tile, causal):
+    """{sequence, first position} of every tile of `tile` queries ("q") or keys ("k"), most work first:
+    the keys its last query sees, or the queries that see its first key."""
+    n = nq if side == "q" else nk
+    count = -(-n // tile)
+    seq = np.repeat(np.arange(len(n)), count)
+    first = (np.arange(len(seq)) - np.repeat(np.cumsum(count) - count, count)) * tile
+    q, k = nq[seq], nk[seq]
+    if side == "q":
+        work = np.clip(first + tile + k - q, 0, k) if causal else k
+    else:
+        work = np.clip(k - first, 0, q) if causal else q
+    order = np.argsort(-work, kind="stable")
+    return np.ascontiguousarray(np.stack([seq[order], first[order]], 1).astype(np.int32))
+
+
 class PackedSequences:
     """Where the sequences of a packed batch lie: `lengths` queries and `key_lengths` keys (default:
     the same) of each, one behind the other.  A sequence's queries are the LAST ones of its keys'
@@ -182,18 +198,8 @@ class PackedSequences:
         key = (side, tile, bool(causal))
         got = self._tables.get(key)
         if got is None:
-            n = self._q if side == "q" else self._k
-            count = -(-n // tile)
-            seq = np.repeat(np.arange(len(n)), count)
-            first = (np.arange(len(seq)) - np.repeat(np.cumsum(count) - count, count)) * tile
-            nq, nk = self._q[seq], self._k[seq]
-            if side == "q":
-                work = np.clip(first + tile + nk - nq, 0, nk) if causal else nk
-            else:
-                work = np.clip(nq - (first - (nk - nq)), 0, nq) if causal else nq
-            order = np.argsort(-work, kind="stable")
-            table = np.ascontiguousarray(np.stack([seq[order], first[order]], 1).astype(np.int32))
-            got = self._tables[key] = (self._upload(table.reshape(-1)) if len(seq) else None, len(seq))
+            table = tile_table(self._q, self._k, side, tile, causal)
+            got = self._tables[key] = (self._upload(table.reshape(-1)) if len(table) else None, len(table))
         return got
 
     def _call(self, type_, Hq, Hkv, D, causal, buckets):
