@@ -576,21 +576,21 @@ int vaesne_pack(const float* const* srcs, const int64_t* offs, const int64_t* ns
 /* ---- attention over packed sequences ----------------------------------------
  * Sequences of different lengths lie one behind the other, without padding: q [total_q, Hq, D],
  * k, v [total_k, Hkv, D] (rows of D unit-stride elements, 16-byte aligned; ts / hs = token / head
- * stride in elements).  Sequence s holds tokens cu_q[s] .. cu_q[s+1] of q and cu_k[s] .. cu_k[s+1]
- * of k, v; its queries are the LAST nq of its nk positions (query i stands at i + nk - nq).
+ * stride in elements).  A sequence's queries are the LAST nq of its nk positions (query i stands at i + nk - nq).
  *   S = scale q k^T + table[lut[clamp(j - i - (nk - nq), -R, R) + R], head]   (table: nullable)
  *   causal: key j is seen iff j <= i + nk - nq;  o = softmax(S) v, 0 where nothing is seen.
  * Query head h reads key head h / (Hq / Hkv).  type: 0 fp32, 1 bf16, 2 fp16 (every tensor but the
  * fp32 statistics has it).  D: a multiple of 8, at most 128.
- * q_tiles / k_tiles: {sequence, first position} of every tile of q_tile positions / k_tile keys, in
- * any order (longest work first is fastest); vaesne_packed_attn_tiles gives q_tile and k_tile. */
+ * q_tiles / k_tiles [n][8]: one row for every tile of q_tile positions / k_tile keys of a sequence, in any
+ * order (longest work first is fastest): {first query token, first key token, queries, keys of the
+ * sequence, first position of the tile, 0, 0, 0}; vaesne_packed_attn_tiles gives q_tile and k_tile. */
 typedef struct vaesne_packed_attn {
   int type, Hq, Hkv, D, causal, num_buckets, max_distance, nseq;
   float scale;                       /* > 0 */
   int max_q, max_k;                  /* longest sequence's queries / keys */
   int q_tile, k_tile, n_q_tiles, n_k_tiles;
   int64_t total_q, total_k;
-  const int32_t *cu_q, *cu_k, *q_tiles, *k_tiles;
+  const int32_t *q_tiles, *k_tiles;
   const void *q, *k, *v;
   int64_t q_ts, q_hs, k_ts, k_hs, v_ts, v_hs;
   void* o;                           /* [total_q, Hq, D] dense (out; in for the backward) */

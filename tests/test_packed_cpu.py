@@ -50,17 +50,19 @@ def test_tile_table_covers_every_position_once_longest_first(side, tile, causal)
     nk = np.array([9, 0, 40, 32, 20, 500, 4000], dtype=np.int64)
     t = _packed_ops.tile_table(nq, nk, side, tile, causal)
     n = nq if side == "q" else nk
-    want = sorted((s, p) for s in range(len(n)) for p in range(0, int(n[s]), tile))
+    q0, k0 = np.cumsum(nq) - nq, np.cumsum(nk) - nk
+    want = sorted((q0[s], k0[s], nq[s], nk[s], p, 0, 0, 0) for s in range(len(n)) for p in range(0, int(n[s]), tile))
     assert sorted(map(tuple, t.tolist())) == want and t.dtype == np.int32
+    which = [[s for s in range(len(n)) if (q0[s], k0[s], nq[s], nk[s]) == tuple(r[:4])][0] for r in t.tolist()]
 
     def work(s, p):
         if side == "q":
             return sum(1 for j in range(nk[s]) if j <= min(p + tile, nq[s]) - 1 + nk[s] - nq[s]) if causal else nk[s]
         return sum(1 for i in range(nq[s]) if p <= i + nk[s] - nq[s]) if causal else nq[s]
-    got = [work(s, p) for s, p in t.tolist()]
+    got = [work(s, r[4]) for s, r in zip(which, t.tolist())]
     # (a last, short tile is ranked as a whole one)
     assert all(b <= a + tile for a, b in zip(got, got[1:]))
-    assert _packed_ops.tile_table(nq[:0], nk[:0], side, tile, causal).shape == (0, 2)
+    assert _packed_ops.tile_table(nq[:0], nk[:0], side, tile, causal).shape == (0, 8)
 
 
 # ---- refusals of the Python entry points ------------------------------------------------------------
@@ -95,7 +97,7 @@ def test_unpack8_takes_only_its_own():
 # ---- refusals at the C entry points -------------------------------------------------------------------
 def attn_args(**kw):
     a = _packed_ops._AttnArgs(type=1, Hq=8, Hkv=2, D=64, causal=1, nseq=1, scale=0.125, max_q=100, max_k=100,
-                              total_q=100, total_k=100, cu_q=64, cu_k=64, q_tiles=64, k_tiles=64, q=64, k=64, v=64,
+                              total_q=100, total_k=100, q_tiles=64, k_tiles=64, q=64, k=64, v=64,
                               q_ts=512, q_hs=64, k_ts=128, k_hs=64, v_ts=128, v_hs=64, o=64, lse=64, dout=64, do_ts=512,
                               do_hs=64, dq=64, dk=64, dv=64, workspace=64, n_q_tiles=4, n_k_tiles=1)
     qt, kt = C.c_int(), C.c_int()
@@ -109,7 +111,7 @@ def attn_args(**kw):
 @pytest.mark.parametrize("change", [
     dict(type=3), dict(type=-1), dict(Hq=0), dict(Hkv=3), dict(Hkv=0), dict(D=0), dict(D=12), dict(D=136),
     dict(scale=0.0), dict(scale=-1.0), dict(scale=math.nan), dict(q_tile=31), dict(k_tile=64), dict(max_q=1 << 26),
-    dict(max_k=1 << 26), dict(total_q=-1), dict(q=None), dict(k=None), dict(o=None), dict(lse=None), dict(cu_q=None),
+    dict(max_k=1 << 26), dict(total_q=-1), dict(q=None), dict(k=None), dict(o=None), dict(lse=None),
     dict(q_tiles=None), dict(n_q_tiles=0), dict(q=72), dict(k=66), dict(q_ts=516), dict(v_hs=4), dict(k_ts=1 << 23),
     dict(q_hs=-64), dict(table=64, max_distance=0, num_buckets=4), dict(table=64, max_distance=513, num_buckets=4),
     dict(table=64, max_distance=8, num_buckets=0), dict(table=64, max_distance=8, num_buckets=4, lut=None)])

@@ -35,7 +35,7 @@ class _AttnArgs(C.Structure):
     _fields_ = _fields([
         (C.c_int, "type Hq Hkv D causal num_buckets max_distance nseq"), (C.c_float, "scale"),
         (C.c_int, "max_q max_k q_tile k_tile n_q_tiles n_k_tiles"), (C.c_int64, "total_q total_k"),
-        (C.c_void_p, "cu_q cu_k q_tiles k_tiles q k v"),
+        (C.c_void_p, "q_tiles k_tiles q k v"),
         (C.c_int64, "q_ts q_hs k_ts k_hs v_ts v_hs"), (C.c_void_p, "o lse table lut dout"),
         (C.c_int64, "do_ts do_hs"), (C.c_void_p, "dq dk dv dtable workspace")])
 
@@ -104,8 +104,9 @@ def _lengths(lengths, name):
 
 
 def tile_table(nq, nk, side, tile, causal):
-    """{sequence, first position} of every tile of `tile` queries ("q") or keys ("k"), most work first:
-    the keys its last query sees, or the queries that see its first key."""
+    """[n][8] rows {first query token, first key token, queries, keys, first position} of every tile of
+    `tile` queries ("q") or keys ("k"), most work first: the keys its last query sees, or the queries that
+    see its first key."""
     n = nq if side == "q" else nk
     count = -(-n // tile)
     seq = np.repeat(np.arange(len(n)), count)
@@ -116,7 +117,9 @@ def tile_table(nq, nk, side, tile, causal):
     else:
         work = np.clip(k - first, 0, q) if causal else q
     order = np.argsort(-work, kind="stable")
-    return np.ascontiguousarray(np.stack([seq[order], first[order]], 1).astype(np.int32))
+    out = np.zeros((len(seq), 8), dtype=np.int32)
+    out[:, :5] = np.stack([(np.cumsum(nq) - nq)[seq], (np.cumsum(nk) - nk)[seq], q, k, first], 1)[order]
+    return out
 
 
 class PackedSequences:
@@ -144,12 +147,6 @@ class PackedSequences:
         self.total, self.total_keys = int(self._q.sum()), int(self._k.sum())
         self.longest = max(self.lengths, default=0)
         self.longest_keys = max(self.key_lengths, default=0)
-        cu = np.zeros(2 * (len(self.lengths) + 1), dtype=np.int32)
-        n = len(self.lengths) + 1
-        cu[1:n] = np.cumsum(self._q)
-        cu[n + 1:] = np.cumsum(self._k)
-        self._cu = self._upload(cu)
-        self._cu_k_ptr = self._cu.data_ptr() + 4 * n
         self._tables = {}
         self._calls = {}
         self._index = None
@@ -194,7 +191,7 @@ class PackedSequences:
         return torch.from_numpy(array).to(self.device)       # (waits for the copy: any stream may read it)
 
     def _table(self, side, tile, causal):
-        """{sequence, first position} of every tile, most work first."""
+        """tile_table's rows on the device, and how many."""
         key = (side, tile, bool(causal))
         got = self._tables.get(key)
         if got is None:
@@ -208,8 +205,7 @@ class PackedSequences:
         got = self._calls.get(key)
         if got is None:
             a = _AttnArgs(type=type_, Hq=Hq, Hkv=Hkv, D=D, causal=int(causal), nseq=len(self.lengths), scale=1.0,
-                          max_q=self.longest, max_k=self.longest_keys, total_q=self.total, total_k=self.total_keys,
-                          cu_q=self._cu.data_ptr(), cu_k=self._cu_k_ptr)
+                          max_q=self.longest, max_k=self.longest_keys, total_q=self.total, total_k=self.total_keys)
             if buckets is not None:
                 a.num_buckets, a.max_distance = buckets.num_buckets, buckets.max_distance
                 a.table = a.dtable = 16                      # (any address: sizes only)
@@ -224,7 +220,7 @@ class PackedSequences:
             if min(ws) < 0:
                 raise RuntimeError("packed_attention: sizes out of range")
             a.table = a.dtable = None
-            got = self._calls[key] = (bytes(a), ws, [t for t in (self._cu, tq, tk) if t is not None])
+            got = self._calls[key] = (bytes(a), ws, [t for t in (tq, tk) if t is not None])
         return got
 
     def _args(self, call):
@@ -289,7 +285,7 @@ def _head_rows(t):
     """t [T, H, D] with unit-stride, 16-byte aligned rows (a copy where it has none)."""
     n = t.element_size()
     s = t.stride()
-    if s[2] == 1 and s[0] * n % 16 == 0 and s[1] * n % 16 == 0 and t.data_ptr() % 16 == 0 and max(s) < 1 << 22:
+    if s[2] == 1 and s[0] * n % 16 == 0 and s[1] * n % 16 == 0 and t.data_ptr() % 16 == 0 and max(s) < 1 << 21:
         return t
     return t.clone(memory_format=torch.contiguous_format)
 

@@ -221,16 +221,17 @@ __device__ __forceinline__ float load_f32(const float* base, uint32_t off) {   /
   return __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rsrc, off, 0, 0));
 }
 
+// a lane's fragments of one row, `off` bytes from `base` (uniform); NO_ROW: zeros
 template <class T, int DP> using Frags = typename Ty<T>::Frag[Tile<T, DP>::NCH];
 template <class T, int DP>
-__device__ __forceinline__ void load_frags(Frags<T, DP>& f, const T* p, int D, int h) {
+__device__ __forceinline__ void load_frags(Frags<T, DP>& f, const T* base, uint32_t off, int D, int h) {
   using L = Tile<T, DP>;
+  const auto rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(base), 0, 0x7fffffff, 0x00020000);
 #pragma unroll
   for (int k = 0; k < L::NCH; ++k) {
     const int d = k * L::KC + h * L::EPC;
-    u4 x{0, 0, 0, 0};
-    if (p != nullptr && d < D) x = *reinterpret_cast<const u4*>(p + d);
-    f[k] = __builtin_bit_cast(typename Ty<T>::Frag, x);
+    f[k] = __builtin_bit_cast(typename Ty<T>::Frag,
+                              __builtin_amdgcn_raw_buffer_load_b128(rsrc, d < D ? off + d * (uint32_t)sizeof(T) : NO_ROW, 0, 0));
   }
 }
 
@@ -251,7 +252,7 @@ __device__ __forceinline__ void store_col(U* p, const f16v (&o)[DT], float f, in
 
 // The bias of every relative position for one head, log2 domain: -R .. R and MARGIN more on either
 // side that repeat the ends, so that a tile which is not wholly beyond +-R reads without clamping.
-constexpr int MARGIN = 64;
+constexpr int MARGIN = 64, SKEW = 2048;
 __host__ __device__ __forceinline__ int span_of(int R) { return 2 * (R + MARGIN) + 1; }
 template <class T, int NT>
 __device__ __forceinline__ void load_bias(const Args& a, float* lut, int head) {
@@ -273,12 +274,12 @@ struct QTile {
   int pos0, nq, nk, npos, nrows, off, kvh, head0;
   int64_t q0, k0;
   __device__ __forceinline__ QTile(const Args& a, int tile, int hidx) {
-    const int seq = uni(a.p.q_tiles[2 * tile]);
-    pos0 = uni(a.p.q_tiles[2 * tile + 1]);
-    q0 = uni(a.p.cu_q[seq]);
-    k0 = uni(a.p.cu_k[seq]);
-    nq = uni(a.p.cu_q[seq + 1]) - (int)q0;
-    nk = uni(a.p.cu_k[seq + 1]) - (int)k0;
+    const int32_t* t = a.p.q_tiles + 8 * (int64_t)tile;
+    q0 = uni(t[0]);
+    k0 = uni(t[1]);
+    nq = uni(t[2]);
+    nk = uni(t[3]);
+    pos0 = uni(t[4]);
     off = nk - nq;
     npos = min(a.p.q_tile, nq - pos0);
     nrows = npos * a.pg;
@@ -290,18 +291,19 @@ struct QTile {
   }
 };
 
-// scores of one 32x32 tile to the log2 domain with bias, s c + bias.  Register r's relative position is
+// scores of one 32x32 tile to the log2 domain with bias, s c + bias + more.  Register r's relative position is
 // rel0 + SIGN acc_row(r, h); lo .. hi (uniform) bounds those of the tile.
 template <int SIGN>
-__device__ __forceinline__ void add_bias(f16v& s, float c, const float* lut, int rel0, int lo, int hi, int h, int R) {
+__device__ __forceinline__ void add_bias(f16v& s, float c, const float* lut, int rel0, int lo, int hi, int h, int R,
+                                         float more = 0.f) {
   if (hi <= -R || lo >= R) {                               // one bucket for the whole tile
-    const float b = lut[hi <= -R ? 0 : 2 * (R + MARGIN)];
+    const float b = lut[hi <= -R ? 0 : 2 * (R + MARGIN)] + more;
 #pragma unroll
     for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], c, b);
   } else {
     const float* p = lut + (rel0 + SIGN * 4 * h + R + MARGIN);
 #pragma unroll
-    for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], c, p[SIGN * acc_row(r, 0)]);
+    for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], c, p[SIGN * acc_row(r, 0)] + more);
   }
 }
 
@@ -334,8 +336,6 @@ __global__ __launch_bounds__(NW * 64, (occ<T, DP, BIAS, NW, false>())) void fwd_
   const int hidx = blockIdx.x % nh;
   const QTile t(a, blockIdx.x / nh, hidx);
   const int lane = threadIdx.x & 63, w = uni(threadIdx.x >> 6), h = lane >> 5, D = a.p.D, R = a.p.max_distance;
-  if (BIAS) load_bias<T, NT>(a, lut, t.head0);
-
   const int row = w * 32 + (lane & 31), dpos = div_pg(a, row);
   const bool valid = row < t.nrows;
   const int head = t.head0 + row - dpos * a.pg;
@@ -346,10 +346,6 @@ __global__ __launch_bounds__(NW * 64, (occ<T, DP, BIAS, NW, false>())) void fwd_
   const int kend = uni(t.limit(a, t.nrows - 1));
   const int nt = (kend + BN - 1) / BN, per = (nt + a.nsplit - 1) / a.nsplit;
   const int t0 = blockIdx.y * per, t1 = min(nt, t0 + per);
-
-  typename Ty<T>::Frag qf[L::NCH];
-  const T* qp = reinterpret_cast<const T*>(a.p.q) + (t.q0 + t.pos0 + dpos) * a.p.q_ts + (int64_t)head * a.p.q_hs;
-  load_frags<T, DP>(qf, valid ? qp : nullptr, D, h);
 
   f16v o[L::DT];
 #pragma unroll
@@ -365,8 +361,13 @@ __global__ __launch_bounds__(NW * 64, (occ<T, DP, BIAS, NW, false>())) void fwd_
     ks.load(kb + (int64_t)j * BN * a.p.k_ts, t.nk - j * BN);
     vs.load(vb + (int64_t)j * BN * a.p.v_ts, t.nk - j * BN);
   };
+  // every load of the prologue is in flight before the first wait
+  if (t0 < t1) fetch(t0);
+  typename Ty<T>::Frag qf[L::NCH];
+  load_frags<T, DP>(qf, reinterpret_cast<const T*>(a.p.q) + (t.q0 + t.pos0) * a.p.q_ts + t.head0 * a.p.q_hs,
+                    valid ? (uint32_t)((dpos * a.p.q_ts + (head - t.head0) * a.p.q_hs) * (int)sizeof(T)) : NO_ROW, D, h);
+  if (BIAS) load_bias<T, NT>(a, lut, t.head0);
   if (t0 < t1) {
-    fetch(t0);
     ks.store(smem);
     vs.store(smem + TILE);
   }
@@ -523,14 +524,12 @@ __global__ __launch_bounds__(NW * 64, (occ<T, DP, BIAS, NW, true>())) void dq_ke
   const int R = a.p.max_distance, NH = 2 * R + 1;
   float* lut = reinterpret_cast<float*>(smem + 4 * TILE);
   float* hist = lut + span_of(R) * (1 + (threadIdx.x >> 6));   // this wave's sums by relative position
+  float* skew = lut + (span_of(R) * (1 + NW) + 3) / 4 * 4 + SKEW * (threadIdx.x >> 6);   // and 32 x 64 to take them
   const int nh = a.p.Hkv * a.nsub;
   const int hidx = blockIdx.x % nh;
   const QTile t(a, blockIdx.x / nh, hidx);
   const int lane = threadIdx.x & 63, w = uni(threadIdx.x >> 6), h = lane >> 5, D = a.p.D;
   const bool sums = BIAS && a.p.dtable != nullptr;
-  if (BIAS) load_bias<T, NT>(a, lut, t.head0);
-  if (sums)
-    for (int i = lane; i < span_of(R); i += 64) hist[i] = 0.f;
 
   const int row = w * 32 + (lane & 31), dpos = div_pg(a, row);
   const bool valid = row < t.nrows;
@@ -544,24 +543,41 @@ __global__ __launch_bounds__(NW * 64, (occ<T, DP, BIAS, NW, true>())) void dq_ke
   const int nt = (kend + BN - 1) / BN, per = (nt + a.nsplit - 1) / a.nsplit;
   const int t0 = blockIdx.y * per, t1 = min(nt, t0 + per);
 
-  const int64_t tok = t.q0 + t.pos0 + dpos, rid = tok * a.p.Hq + head;
-  typename Ty<T>::Frag qf[L::NCH], gf[L::NCH];
-  load_frags<T, DP>(qf, valid ? reinterpret_cast<const T*>(a.p.q) + tok * a.p.q_ts + (int64_t)head * a.p.q_hs : nullptr, D, h);
-  load_frags<T, DP>(gf, valid ? reinterpret_cast<const T*>(a.p.dout) + tok * a.p.do_ts + (int64_t)head * a.p.do_hs : nullptr, D, h);
-  float delta = 0.f, big = 0.f;
-  {
-    typename Ty<T>::Frag of[L::NCH];
-    load_frags<T, DP>(of, valid ? reinterpret_cast<const T*>(a.p.o) + rid * D : nullptr, D, h);
-#pragma unroll
-    for (int k = 0; k < L::NCH; ++k)
-#pragma unroll
-      for (int e = 0; e < L::EPC; ++e) {
-        delta = fmaf((float)gf[k][e], (float)of[k][e], delta);
-        if (HALF) big = fmaxf(big, fabsf((float)gf[k][e]));
-      }
+  const T* kb = reinterpret_cast<const T*>(a.p.k) + t.k0 * a.p.k_ts + t.kvh * a.p.k_hs;
+  const T* vb = reinterpret_cast<const T*>(a.p.v) + t.k0 * a.p.v_ts + t.kvh * a.p.v_hs;
+  Stage<T, DP, BN, NT> ks, vs;
+  ks.init(D, [&](int r) { return (uint32_t)r * (uint32_t)(a.p.k_ts * sizeof(T)); });
+  vs.init(D, [&](int r) { return (uint32_t)r * (uint32_t)(a.p.v_ts * sizeof(T)); });
+  auto fetch = [&](int j) {
+    ks.load(kb + (int64_t)j * BN * a.p.k_ts, t.nk - j * BN);
+    vs.load(vb + (int64_t)j * BN * a.p.v_ts, t.nk - j * BN);
+  };
+  if (t0 < t1) fetch(t0);
+  const int64_t tok0 = t.q0 + t.pos0, rid0 = tok0 * a.p.Hq + t.head0;
+  const int rofs = dpos * a.p.Hq + head - t.head0;
+  const int64_t rid = rid0 + rofs;
+  typename Ty<T>::Frag qf[L::NCH], gf[L::NCH], of[L::NCH];
+  load_frags<T, DP>(qf, reinterpret_cast<const T*>(a.p.q) + tok0 * a.p.q_ts + t.head0 * a.p.q_hs,
+                    valid ? (uint32_t)((dpos * a.p.q_ts + (head - t.head0) * a.p.q_hs) * (int)sizeof(T)) : NO_ROW, D, h);
+  load_frags<T, DP>(gf, reinterpret_cast<const T*>(a.p.dout) + tok0 * a.p.do_ts + t.head0 * a.p.do_hs,
+                    valid ? (uint32_t)((dpos * a.p.do_ts + (head - t.head0) * a.p.do_hs) * (int)sizeof(T)) : NO_ROW, D, h);
+  load_frags<T, DP>(of, reinterpret_cast<const T*>(a.p.o) + rid0 * D, valid ? (uint32_t)(rofs * D * (int)sizeof(T)) : NO_ROW, D, h);
+  const float lse_in = load_f32(a.p.lse + rid0, valid ? 4u * rofs : NO_ROW);
+  if (BIAS) load_bias<T, NT>(a, lut, t.head0);
+  if (sums) {
+    for (int i = lane; i < span_of(R); i += 64) hist[i] = 0.f;
+    for (int i = lane; i < SKEW; i += 64) skew[i] = 0.f;
   }
+  const float lse = valid ? lse_in : INF;
+  float delta = 0.f, big = 0.f;
+#pragma unroll
+  for (int k = 0; k < L::NCH; ++k)
+#pragma unroll
+    for (int e = 0; e < L::EPC; ++e) {
+      delta = fmaf((float)gf[k][e], (float)of[k][e], delta);
+      if (HALF) big = fmaxf(big, fabsf((float)gf[k][e]));
+    }
   delta = xsum32(delta);
-  const float lse = valid ? a.p.lse[rid] : INF;
   float up = 1.f;                                              // 1 / (the factor on dS)
   if (HALF) {
     big = xmax32(big);
@@ -573,23 +589,17 @@ __global__ __launch_bounds__(NW * 64, (occ<T, DP, BIAS, NW, true>())) void dq_ke
   }
   const float down = 1.f / up;
   if (valid && h == 0 && blockIdx.y == 0) a.delta[rid] = delta;
+  // dP starts from -delta where the registers allow a copy of it (one subtraction less per score)
+  constexpr bool FROM = DP <= 64;
+  f16v minus;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) minus[r] = FROM ? -delta : 0.f;
 
   f16v o[L::DT];
 #pragma unroll
   for (int i = 0; i < L::DT; ++i) o[i] = f16v{};
   float far_lo = 0.f, far_hi = 0.f;
-
-  const T* kb = reinterpret_cast<const T*>(a.p.k) + t.k0 * a.p.k_ts + t.kvh * a.p.k_hs;
-  const T* vb = reinterpret_cast<const T*>(a.p.v) + t.k0 * a.p.v_ts + t.kvh * a.p.v_hs;
-  Stage<T, DP, BN, NT> ks, vs;
-  ks.init(D, [&](int r) { return (uint32_t)r * (uint32_t)(a.p.k_ts * sizeof(T)); });
-  vs.init(D, [&](int r) { return (uint32_t)r * (uint32_t)(a.p.v_ts * sizeof(T)); });
-  auto fetch = [&](int j) {
-    ks.load(kb + (int64_t)j * BN * a.p.k_ts, t.nk - j * BN);
-    vs.load(vb + (int64_t)j * BN * a.p.v_ts, t.nk - j * BN);
-  };
   if (t0 < t1) {
-    fetch(t0);
     ks.store(smem);
     vs.store(smem + TILE);
   }
@@ -605,7 +615,7 @@ __global__ __launch_bounds__(NW * 64, (occ<T, DP, BIAS, NW, true>())) void dq_ke
     for (int n = 0; n < NB; ++n) {
       const int base = j * BN + 32 * n;
       if (base < wmax) {
-        f16v s = f16v{}, g = f16v{};
+        f16v s = f16v{}, g = minus;
 #pragma unroll
         for (int k = 0; k < L::NCH; ++k) s = mma(L::row(K, at, 32 * n, k), qf[k], s);
 #pragma unroll
@@ -614,9 +624,9 @@ __global__ __launch_bounds__(NW * 64, (occ<T, DP, BIAS, NW, true>())) void dq_ke
         const float c = BIAS ? 1.f : a.c;
         const int rel0 = base - qabs;
         const int lo = base - qfirst - 31, hi = base - qfirst + 31;   // the tile's relative positions
-        if (BIAS) add_bias<1>(s, a.c, lut, rel0, lo, hi, h, R);
+        if (BIAS) add_bias<1>(s, a.c, lut, rel0, lo, hi, h, R, -lse);
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c, -lse)) * (g[r] - delta);
+        for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c, BIAS ? 0.f : -lse)) * (FROM ? g[r] : g[r] - delta);
         if (base + 32 > wmin) {
 #pragma unroll
           for (int r = 0; r < 16; ++r)
@@ -630,17 +640,19 @@ __global__ __launch_bounds__(NW * 64, (occ<T, DP, BIAS, NW, true>())) void dq_ke
 #pragma unroll
             for (int r = 0; r < 16; ++r) far_hi += s[r];
           } else {
-            // one half of the wave at a time: the 32 lanes of a half meet 32 different distances in
-            // each register and a wave's LDS operations keep their order, so every sum of this
-            // wave-private array is taken in one fixed order
-            float* p = hist + (rel0 + 4 * h + R + MARGIN);
-            for (int half = 0; half < 2; ++half) {
-              if (h == half) {
+            // Row i's keys are written i places further left, so that a column holds one distance: lane d
+            // sums column d over the 32 rows and adds it to this wave's sums.  (A wave's LDS operations
+            // keep their order; places that no key reaches stay zero.  Adding each score atomically took
+            // 280 cycles for 32 of them: 145 us instead of XXX, fp16 training with 12 heads of 64.)
+            float* p = skew + 63 * (lane & 31) + 4 * h + 31;
 #pragma unroll
-                for (int r = 0; r < 16; ++r)
-                  __hip_atomic_fetch_add(p + acc_row(r, 0), s[r], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WAVEFRONT);
-              }
-            }
+            for (int r = 0; r < 16; ++r) p[acc_row(r, 0)] = s[r];
+            float x = 0.f;
+#pragma unroll
+            for (int i = 0; i < 32; ++i) x += skew[64 * i + lane];
+            // column d: distance base - qfirst + d - 31; column 63 holds nothing
+            float* q = hist + (lo + lane + R + MARGIN);
+            *q += x;
           }
         }
         if (HALF) {
@@ -720,26 +732,29 @@ __global__ __launch_bounds__(NW * 64, (occ_kv<T, DP, NW>())) void dkv_kernel(Arg
   constexpr int NT = NW * 64, BQ = row_tile<T, DP>(), NB = BQ / 32, TILE = BQ * L::RB;
   constexpr bool VL = v_in_lds<T, DP>(), HALF = __is_same(T, _Float16);
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  float* stat = reinterpret_cast<float*>(smem + 4 * TILE);     // [2][lse BQ | delta BQ]
+  float* stat = reinterpret_cast<float*>(smem + 4 * TILE);     // [2][lse BQ | -delta BQ]
   float* lut = stat + 4 * BQ;
   char* vt = smem + 4 * TILE + 16 * BQ + (BIAS ? (span_of(a.p.max_distance) * 4 + 15) / 16 * 16 : 0);   // this tile's V (VL)
   const int kvh = blockIdx.x % a.p.Hkv, tile = blockIdx.x / a.p.Hkv, D = a.p.D, R = a.p.max_distance;
-  const int seq = uni(a.p.k_tiles[2 * tile]), key0 = uni(a.p.k_tiles[2 * tile + 1]);
-  const int64_t q0 = uni(a.p.cu_q[seq]), k0 = uni(a.p.cu_k[seq]);
-  const int nq = uni(a.p.cu_q[seq + 1]) - (int)q0, nk = uni(a.p.cu_k[seq + 1]) - (int)k0, off = nk - nq;
+  const int32_t* tl = a.p.k_tiles + 8 * (int64_t)tile;
+  const int64_t q0 = uni(tl[0]), k0 = uni(tl[1]);
+  const int nq = uni(tl[2]), nk = uni(tl[3]), key0 = uni(tl[4]), off = nk - nq;
   const int lane = threadIdx.x & 63, w = uni(threadIdx.x >> 6), h = lane >> 5;
   const int key = key0 + w * 32 + (lane & 31);
   const bool valid = key < nk;
   typename Ty<T>::Frag kf[L::NCH], vf[VL ? 1 : L::NCH];
-  load_frags<T, DP>(kf, valid ? reinterpret_cast<const T*>(a.p.k) + (k0 + key) * a.p.k_ts + kvh * a.p.k_hs : nullptr, D, h);
-  const T* vp = reinterpret_cast<const T*>(a.p.v) + (k0 + key) * a.p.v_ts + kvh * a.p.v_hs;
+  const int kr = w * 32 + (lane & 31);
+  const T* vp = reinterpret_cast<const T*>(a.p.v) + (k0 + key0) * a.p.v_ts + kvh * a.p.v_hs;
+  const uint32_t vofs = valid ? (uint32_t)(kr * a.p.v_ts * (int)sizeof(T)) : NO_ROW;
+  load_frags<T, DP>(kf, reinterpret_cast<const T*>(a.p.k) + (k0 + key0) * a.p.k_ts + kvh * a.p.k_hs,
+                    valid ? (uint32_t)(kr * a.p.k_ts * (int)sizeof(T)) : NO_ROW, D, h);
   if constexpr (VL) {
     typename Ty<T>::Frag f[L::NCH];                            // each wave writes and reads its own 32 rows
-    load_frags<T, DP>(f, valid ? vp : nullptr, D, h);
+    load_frags<T, DP>(f, vp, vofs, D, h);
 #pragma unroll
     for (int k = 0; k < L::NCH; ++k) *reinterpret_cast<typename Ty<T>::Frag*>(vt + L::at(w * 32 + (lane & 31), 2 * k + h)) = f[k];
   } else {
-    load_frags<T, DP>(vf, valid ? vp : nullptr, D, h);
+    load_frags<T, DP>(vf, vp, vofs, D, h);
   }
   f16v dk[L::DT], dv[L::DT];
 #pragma unroll
@@ -786,7 +801,7 @@ __global__ __launch_bounds__(NW * 64, (occ_kv<T, DP, NW>())) void dkv_kernel(Arg
     gs.store(smem + b * 2 * TILE + TILE);
     if (threadIdx.x < BQ) {
       stat[b * 2 * BQ + threadIdx.x] = st_in ? st_l : INF;
-      stat[b * 2 * BQ + BQ + threadIdx.x] = st_d;
+      stat[b * 2 * BQ + BQ + threadIdx.x] = -st_d;
     }
   };
   int sub_now = -1;
@@ -847,7 +862,12 @@ __global__ __launch_bounds__(NW * 64, (occ_kv<T, DP, NW>())) void dkv_kernel(Arg
         }
         feed<L::DT * L::TB, L::CR, 3>();
         __builtin_amdgcn_sched_barrier(0);                     // (merged with the next stage it spills)
-        g[n] = f16v{};
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {                          // dP starts from -delta
+          const f4 x = *reinterpret_cast<const f4*>(dl + 32 * n + 8 * q + 4 * h);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) g[n][4 * q + e] = x[e];
+        }
 #pragma unroll
         for (int k = 0; k < L::NCH; ++k) {
           if constexpr (VL) g[n] = mma(L::row(G, at, 32 * n, k), L::row(vt, at, w * 32, k), g[n]);
@@ -856,11 +876,7 @@ __global__ __launch_bounds__(NW * 64, (occ_kv<T, DP, NW>())) void dkv_kernel(Arg
         feed<L::NCH, VL ? 2 : 1, VL ? 2 : 3>();
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const f4 x = *reinterpret_cast<const f4*>(dl + 32 * n + 8 * q + 4 * h);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) s[n][4 * q + e] *= (g[n][4 * q + e] - x[e]) * (HALF ? down : 1.f);
-        }
+        for (int r = 0; r < 16; ++r) s[n][r] *= HALF ? g[n][r] * down : g[n][r];
 #pragma unroll
         for (int t = 0; t < L::TB; ++t) {
           const auto sf = take<T>(s[n], t);
@@ -936,7 +952,8 @@ template <class T, int DP, bool BIAS> int bwd_dp(const Plan& p, hipStream_t s) {
   if (a.p.n_q_tiles > 0) {
     a.nsplit = p.split_q;
     const int wgs = a.p.n_q_tiles * a.p.Hkv * a.nsub;
-    const size_t lds = 4 * BN * RB + (BIAS ? (1 + p.nwq) * span_of(a.p.max_distance) * 4 : 0);
+    const size_t lds = 4 * BN * RB + (BIAS ? ((1 + p.nwq) * span_of(a.p.max_distance) + 3) / 4 * 16 : 0) +
+                       (BIAS && a.p.dtable ? p.nwq * SKEW * 4 : 0);
     const int rc = p.nwq == 2 ? launch<T>(dq_kernel<T, DP, BIAS, 2>, dim3(wgs, a.nsplit), 128, lds, a, s)
                               : launch<T>(dq_kernel<T, DP, BIAS, 4>, dim3(wgs, a.nsplit), 256, lds, a, s);
     if (rc) return rc;

@@ -42,7 +42,7 @@ namespace {
 constexpr int SLOTS = 512;            // workgroups the chip runs at once: two of 64 KB LDS per CU
 constexpr int MAX_SPLIT = 64;
 constexpr int64_t MAX_PART = 256 << 20;
-constexpr int64_t MAX_STRIDE = 1 << 22;  // elements: a tile of 64 rows spans less than 2^31 bytes
+constexpr int64_t MAX_STRIDE = 1 << 21;  // elements: a tile of 128 rows spans less than 2^31 bytes
 constexpr int64_t MAX_ROWS = 1 << 25; // rows of one sequence: 32-bit row arithmetic with room
 
 // Parts to cut the streamed axis into.  Each of `wgs` workgroups walks up to `longest` tiles, `mean` on
@@ -155,7 +155,6 @@ int check(const Plan& p, int64_t bytes, int backward) {
   const vaesne_packed_attn& a = p.a.p;
   const int size = a.type == 0 ? 4 : 2;
   const int bad = (int)hipErrorInvalidValue;
-  if (!a.cu_q || !a.cu_k) return bad;
   if (a.q_tile != p.nwq * 32 / p.a.pg || a.k_tile != p.nwk * 32) return bad;
   if (a.n_q_tiles < 0 || a.n_k_tiles < 0 || (a.total_q > 0 && (a.n_q_tiles == 0 || !a.q_tiles || !a.q || !a.o || !a.lse)) ||
       (a.total_k > 0 && (!a.k || !a.v)))
