@@ -602,8 +602,9 @@ typedef struct vaesne_packed_attn {
   void *dq, *dk, *dv, *dtable;       /* dense, the inputs' shapes and type; dtable nullable */
   void* workspace;                   /* vaesne_packed_attn_workspace bytes, 16-byte aligned */
 } vaesne_packed_attn;
-/* q_tile and k_tile for heads, head_dim, type, max_q and max_k of `a`. */
-int vaesne_packed_attn_tiles(const vaesne_packed_attn* a, int* q_tile, int* k_tile);
+/* q_tile and k_tile (backward only) for heads, head_dim, type, max_q and max_k of `a`; the forward's and
+ * the backward's q_tile may differ. */
+int vaesne_packed_attn_tiles(const vaesne_packed_attn* a, int backward, int* q_tile, int* k_tile);
 /* Workspace bytes of the forward (backward = 0) or backward; a negative value: the sizes are refused. */
 int64_t vaesne_packed_attn_workspace(const vaesne_packed_attn* a, int backward);
 int vaesne_packed_attn_fwd(const vaesne_packed_attn* a, void* stream);

@@ -95,13 +95,13 @@ def test_unpack8_takes_only_its_own():
 
 
 # ---- refusals at the C entry points -------------------------------------------------------------------
-def attn_args(**kw):
+def attn_args(backward=0, **kw):
     a = _packed_ops._AttnArgs(type=1, Hq=8, Hkv=2, D=64, causal=1, nseq=1, scale=0.125, max_q=100, max_k=100,
                               total_q=100, total_k=100, q_tiles=64, k_tiles=64, q=64, k=64, v=64,
                               q_ts=512, q_hs=64, k_ts=128, k_hs=64, v_ts=128, v_hs=64, o=64, lse=64, dout=64, do_ts=512,
                               do_hs=64, dq=64, dk=64, dv=64, workspace=64, n_q_tiles=4, n_k_tiles=1)
     qt, kt = C.c_int(), C.c_int()
-    assert _lib.load().vaesne_packed_attn_tiles(C.addressof(a), C.byref(qt), C.byref(kt)) == 0
+    assert _lib.load().vaesne_packed_attn_tiles(C.addressof(a), backward, C.byref(qt), C.byref(kt)) == 0
     a.q_tile, a.k_tile = qt.value, kt.value
     for k, v in kw.items():
         setattr(a, k, v)
@@ -117,15 +117,15 @@ def attn_args(**kw):
     dict(table=64, max_distance=8, num_buckets=0), dict(table=64, max_distance=8, num_buckets=4, lut=None)])
 def test_attention_entry_refuses(change):
     lib = _lib.load()
-    a = attn_args(**change)
-    assert lib.vaesne_packed_attn_fwd(C.addressof(a), None) == BAD
-    assert lib.vaesne_packed_attn_bwd(C.addressof(a), None) == BAD
+    if "k_tile" not in change:
+        assert lib.vaesne_packed_attn_fwd(C.addressof(attn_args(0, **change)), None) == BAD
+    assert lib.vaesne_packed_attn_bwd(C.addressof(attn_args(1, **change)), None) == BAD
 
 
 @pytest.mark.parametrize("change", [dict(dout=None), dict(dq=None), dict(dk=None), dict(dv=None), dict(workspace=None),
                                     dict(workspace=68), dict(k_tiles=None), dict(n_k_tiles=0), dict(do_hs=2)])
 def test_attention_backward_entry_refuses(change):
-    a = attn_args(**change)
+    a = attn_args(1, **change)
     assert _lib.load().vaesne_packed_attn_bwd(C.addressof(a), None) == BAD
 
 

@@ -116,7 +116,7 @@ SIGNATURES = {
     "vaesne_loss_stat": (I32, [P, F32, P, P, P]),
     "vaesne_pack": (I32, [PP, C.POINTER(I64), C.POINTER(I64), I32, P, I32, P]),
     "vaesne_cat": (I32, [PP, C.POINTER(I64), I32, I64, P, P]),
-    "vaesne_packed_attn_tiles": (I32, [P, C.POINTER(I32), C.POINTER(I32)]),
+    "vaesne_packed_attn_tiles": (I32, [P, I32, C.POINTER(I32), C.POINTER(I32)]),
     "vaesne_packed_attn_workspace": (I64, [P, I32]),
     "vaesne_packed_attn_fwd": (I32, [P, P]),
     "vaesne_packed_attn_bwd": (I32, [P, P]),

@@ -199,9 +199,9 @@ class PackedSequences:
             got = self._tables[key] = (self._upload(table.reshape(-1)) if len(table) else None, len(table))
         return got
 
-    def _call(self, type_, Hq, Hkv, D, causal, buckets):
-        """The sizes, tables and workspace bytes of one shape of call, with the struct's plan fields."""
-        key = (type_, Hq, Hkv, D, causal, None if buckets is None else (buckets.num_buckets, buckets.max_distance))
+    def _call(self, type_, Hq, Hkv, D, causal, buckets, backward):
+        """One shape of call: the struct's plan fields, the workspace bytes, the device tables."""
+        key = (type_, Hq, Hkv, D, causal, buckets and (buckets.num_buckets, buckets.max_distance), backward)
         got = self._calls.get(key)
         if got is None:
             a = _AttnArgs(type=type_, Hq=Hq, Hkv=Hkv, D=D, causal=int(causal), nseq=len(self.lengths), scale=1.0,
@@ -210,17 +210,18 @@ class PackedSequences:
                 a.num_buckets, a.max_distance = buckets.num_buckets, buckets.max_distance
                 a.table = a.dtable = 16                      # (any address: sizes only)
             qt, kt = C.c_int(), C.c_int()
-            lib.packed_attn_tiles(C.addressof(a), C.byref(qt), C.byref(kt))
+            lib.packed_attn_tiles(C.addressof(a), int(backward), C.byref(qt), C.byref(kt))
             a.q_tile, a.k_tile = qt.value, kt.value
-            tq, a.n_q_tiles = self._table("q", a.q_tile, causal)
-            tk, a.n_k_tiles = self._table("k", a.k_tile, causal)
-            a.q_tiles = None if tq is None else tq.data_ptr()
-            a.k_tiles = None if tk is None else tk.data_ptr()
-            ws = [lib.packed_attn_workspace(C.addressof(a), b) for b in (0, 1)]
-            if min(ws) < 0:
+            tables = [self._table("q", a.q_tile, causal)]
+            a.q_tiles, a.n_q_tiles = None if tables[0][0] is None else tables[0][0].data_ptr(), tables[0][1]
+            if backward:
+                tables.append(self._table("k", a.k_tile, causal))
+                a.k_tiles, a.n_k_tiles = None if tables[1][0] is None else tables[1][0].data_ptr(), tables[1][1]
+            ws = lib.packed_attn_workspace(C.addressof(a), int(backward))
+            if ws < 0:
                 raise RuntimeError("packed_attention: sizes out of range")
             a.table = a.dtable = None
-            got = self._calls[key] = (bytes(a), ws, [t for t in (tq, tk) if t is not None])
+            got = self._calls[key] = (bytes(a), ws, [t for t, _ in tables if t is not None])
         return got
 
     def _args(self, call):
@@ -295,7 +296,7 @@ def _attn_fwd(q, k, v, seqs, call, scale, table, lut):
     a.scale = scale
     o = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device)
-    ws = _ws(call[1][0], q.device)
+    ws = _ws(call[1], q.device)
     a.q, a.k, a.v = q.data_ptr(), k.data_ptr(), v.data_ptr()
     a.q_ts, a.q_hs, _ = q.stride()
     a.k_ts, a.k_hs, _ = k.stride()
@@ -309,11 +310,11 @@ def _attn_fwd(q, k, v, seqs, call, scale, table, lut):
 
 class PackedAttnFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, v, table, seqs, call, scale, lut):
+    def forward(ctx, q, k, v, table, seqs, call, back, scale, lut):
         _defer.count_uses(*([] if table is None else [table]))
         tab = None if table is None else table.contiguous()
         o, lse = _attn_fwd(q, k, v, seqs, call, scale, tab, lut)
-        ctx.seqs, ctx.call, ctx.scale, ctx.lut = seqs, call, scale, lut
+        ctx.seqs, ctx.back, ctx.scale, ctx.lut = seqs, back, scale, lut
         ctx.save_for_backward(q, k, v, o, lse, tab)
         return o
 
@@ -322,10 +323,10 @@ class PackedAttnFn(torch.autograd.Function):
     def backward(ctx, do):
         q, k, v, o, lse, table = ctx.saved_tensors
         do = _head_rows(do)
-        a = ctx.seqs._args(ctx.call)
+        a = ctx.seqs._args(ctx.back)
         a.scale = ctx.scale
         dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
-        ws = _ws(ctx.call[1][1], q.device)
+        ws = _ws(ctx.back[1], q.device)
         a.q, a.k, a.v = q.data_ptr(), k.data_ptr(), v.data_ptr()
         a.q_ts, a.q_hs, _ = q.stride()
         a.k_ts, a.k_hs, _ = k.stride()
@@ -341,7 +342,7 @@ class PackedAttnFn(torch.autograd.Function):
                 a.dtable = dtable.data_ptr()
         _lib_call("packed_attn_bwd", q.device, C.addressof(a))
         ng = ctx.needs_input_grad
-        return dq if ng[0] else None, dk if ng[1] else None, dv if ng[2] else None, dtable, None, None, None, None
+        return dq if ng[0] else None, dk if ng[1] else None, dv if ng[2] else None, dtable, None, None, None, None, None
 
 
 def packed_attention(q, k, v, seqs, causal=False, scale=None, bias=None, buckets=None):
@@ -374,10 +375,12 @@ def packed_attention(q, k, v, seqs, causal=False, scale=None, bias=None, buckets
                              f"{tuple(bias.shape)}")
         lut = buckets.on(q.device)
     q, k, v = _head_rows(q), _head_rows(k), _head_rows(v)
-    call = seqs._call(type_, Hq, Hkv, D, bool(causal), buckets)
+    causal = bool(causal)
+    call = seqs._call(type_, Hq, Hkv, D, causal, buckets, False)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or
                                     (bias is not None and bias.requires_grad)):
-        return PackedAttnFn.apply(q, k, v, bias, seqs, call, scale, lut)
+        back = seqs._call(type_, Hq, Hkv, D, causal, buckets, True)
+        return PackedAttnFn.apply(q, k, v, bias, seqs, call, back, scale, lut)
     return _attn_fwd(q, k, v, seqs, call, scale, None if bias is None else bias.contiguous(), lut)[0]
 
 

@@ -54,13 +54,16 @@ struct Args {
   int pg, nsub, group;         // heads per tile, tiles per key head's group, query heads per key head
   int pk_log, nsubk;           // dK / dV: log2(heads per row tile), tiles per group
   uint32_t pgm;                // ceil(2^32 / pg), 0 for pg = 1
-  int nsplit;
+  int split_q, split_k;        // parts of the keys (forward, dQ), of the query rows (dK / dV)
+  int per_q, per_k;            // tiles of a part: the same for every sequence, short ones have fewer parts
+  int wgs_q, wgs_k;            // workgroups of a part
   float c;                     // scale * log2(e)
-  float* part;                 // split parts: [nsplit][rows][D] (dK / dV: dk parts, then dv parts)
-  float* part_lse;             // [nsplit][rows]
+  float* part;                 // the forward's or dQ's parts: [split_q][rows][D]
+  float* part_k;               // dk parts [split_k][rows][D], then dv parts
+  float* part_lse;             // [split_q][rows]
   float* delta;                // [total_q][Hq]: rowsum(dO O)
   float* hist;                 // [dQ workgroups][2R + 1]
-  uint32_t* domax;             // [Hkv]: bits of max |dO| (fp16)
+  float *wgmax, *domax;        // fp16: max |dO| of delta_kernel's workgroups, of each key head [Hkv]
 };
 
 __device__ __forceinline__ int div_pg(const Args& a, int row) {
@@ -311,23 +314,22 @@ __device__ __forceinline__ void add_bias(f16v& s, float c, const float* lut, int
 // forward
 // -------------------------------------------------------------------------------------------
 template <class T, int DP> constexpr int key_tile() { return sizeof(T) == 2 ? 64 : 32; }
-// waves per SIMD the registers are budgeted for.  One (all 512 registers) where two would spill: dK /
-// dV at head_dim 128 hold 128 registers of sums beside 64 of operands (two waves, spilling: 1.50 ms,
-// one: 0.73 ms, causal training step of 10 k tokens, 16 heads over 4), fp32 twice the operands,
-// and two-wave workgroups stage twice as much per thread (their LDS allows one wave per SIMD anyway).
-template <class T, int DP, bool BIAS, int NW, bool DQ> constexpr int occ() {
-  return DP == 128 && (sizeof(T) == 4 || NW == 2 || (DQ && BIAS)) ? 1 : 2;
-}
 // dK / dV at head_dim 128 hold 128 registers of sums: V goes to LDS and the row tile is 32, so that two
 // waves per SIMD fit (causal training step of 10 k tokens, 16 heads over 4: V in registers at one
-// wave 0.59 ms, at two, spilling, 1.50 ms; so 0.53 ms)
+// wave 0.59 ms, at two, spilling, 1.50 ms; so 0.50 ms)
 template <class T, int DP> constexpr bool v_in_lds() { return sizeof(T) == 2 && DP == 128; }
-template <class T, int DP, int NW> constexpr int occ_kv() { return (sizeof(T) == 4 && DP >= 64) || (NW == 2 && DP == 128) ? 1 : 2; }
+// waves per SIMD the registers are budgeted for.  One (all 512 registers) where two would spill: fp32 at
+// wide heads, and two-wave workgroups at head_dim 128, which stage twice as much per thread (their LDS
+// allows one wave per SIMD anyway).
+template <class T, int DP, int NW> constexpr int occ_fwd() { return DP == 128 && (sizeof(T) == 4 || NW == 2) ? 1 : 2; }
+template <class T, int DP, bool BIAS, int NW> constexpr int occ_bwd() {
+  return (sizeof(T) == 4 && DP >= 64) || (DP == 128 && (NW == 2 || BIAS)) ? 1 : 2;
+}
 // query rows of a tile in dK / dV
 template <class T, int DP> constexpr int row_tile() { return v_in_lds<T, DP>() ? 32 : key_tile<T, DP>(); }
 
 template <class T, int DP, bool BIAS, int NW>
-__global__ __launch_bounds__(NW * 64, (occ<T, DP, BIAS, NW, false>())) void fwd_kernel(Args a) {
+__global__ __launch_bounds__(NW * 64, (occ_fwd<T, DP, NW>())) void fwd_kernel(Args a) {
   using L = Tile<T, DP>;
   constexpr int NT = NW * 64, BN = key_tile<T, DP>(), NB = BN / 32, TILE = BN * L::RB;
   extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -344,8 +346,7 @@ __global__ __launch_bounds__(NW * 64, (occ<T, DP, BIAS, NW, false>())) void fwd_
   const bool active = w * 32 < t.nrows;
   const int wmin = uni(t.limit(a, w * 32)), wmax = active ? uni(t.limit(a, min(w * 32 + 31, t.nrows - 1))) : 0;
   const int kend = uni(t.limit(a, t.nrows - 1));
-  const int nt = (kend + BN - 1) / BN, per = (nt + a.nsplit - 1) / a.nsplit;
-  const int t0 = blockIdx.y * per, t1 = min(nt, t0 + per);
+  const int nt = (kend + BN - 1) / BN, t0 = blockIdx.y * a.per_q, t1 = min(nt, t0 + a.per_q);
 
   f16v o[L::DT];
 #pragma unroll
@@ -453,12 +454,12 @@ __global__ __launch_bounds__(NW * 64, (occ<T, DP, BIAS, NW, false>())) void fwd_
   const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);      // (a NaN sum stays one)
   const float lse = l == 0.f ? INF : fmaf(m, BIAS ? 1.f : a.c, __log2f(l));
   const int64_t rid = (t.q0 + t.pos0 + dpos) * a.p.Hq + head;
-  if (a.nsplit == 1) {
+  if (a.split_q == 1) {
     store_col(reinterpret_cast<T*>(a.p.o) + rid * D, o, inv, D, h);
     if (h == 0) a.p.lse[rid] = lse;
   } else {
     const int64_t pid = (int64_t)blockIdx.y * a.p.total_q * a.p.Hq + rid;
-    store_col(a.part + pid * D, o, inv, D, h);
+    if (t0 < t1) store_col(a.part + pid * D, o, inv, D, h);    // (the join reads no part that saw nothing)
     if (h == 0) a.part_lse[pid] = lse;
   }
 }
@@ -516,18 +517,19 @@ __device__ __forceinline__ float pow2_of(uint32_t bits) {   // 2^e of |x|, 1 for
 }
 
 template <class T, int DP, bool BIAS, int NW>
-__global__ __launch_bounds__(NW * 64, (occ<T, DP, BIAS, NW, true>())) void dq_kernel(Args a) {
+__device__ __forceinline__ void dq_body(const Args& a, int wg, int part_no) {
   using L = Tile<T, DP>;
   constexpr int NT = NW * 64, BN = key_tile<T, DP>(), NB = BN / 32, TILE = BN * L::RB;
   constexpr bool HALF = __is_same(T, _Float16);
   extern __shared__ __attribute__((aligned(16))) char smem[];
+  const int nsplit = a.split_q;
   const int R = a.p.max_distance, NH = 2 * R + 1;
   float* lut = reinterpret_cast<float*>(smem + 4 * TILE);
   float* hist = lut + span_of(R) * (1 + (threadIdx.x >> 6));   // this wave's sums by relative position
   float* skew = lut + (span_of(R) * (1 + NW) + 3) / 4 * 4 + SKEW * (threadIdx.x >> 6);   // and 32 x 64 to take them
   const int nh = a.p.Hkv * a.nsub;
-  const int hidx = blockIdx.x % nh;
-  const QTile t(a, blockIdx.x / nh, hidx);
+  const int hidx = wg % nh;
+  const QTile t(a, wg / nh, hidx);
   const int lane = threadIdx.x & 63, w = uni(threadIdx.x >> 6), h = lane >> 5, D = a.p.D;
   const bool sums = BIAS && a.p.dtable != nullptr;
 
@@ -540,8 +542,7 @@ __global__ __launch_bounds__(NW * 64, (occ<T, DP, BIAS, NW, true>())) void dq_ke
   const int wmin = w * 32 + 31 < t.nrows ? uni(t.limit(a, w * 32)) : 0;
   const int wmax = active ? uni(t.limit(a, min(w * 32 + 31, t.nrows - 1))) : 0;
   const int kend = uni(t.limit(a, t.nrows - 1));
-  const int nt = (kend + BN - 1) / BN, per = (nt + a.nsplit - 1) / a.nsplit;
-  const int t0 = blockIdx.y * per, t1 = min(nt, t0 + per);
+  const int nt = (kend + BN - 1) / BN, t0 = part_no * a.per_q, t1 = min(nt, t0 + a.per_q);
 
   const T* kb = reinterpret_cast<const T*>(a.p.k) + t.k0 * a.p.k_ts + t.kvh * a.p.k_hs;
   const T* vb = reinterpret_cast<const T*>(a.p.v) + t.k0 * a.p.v_ts + t.kvh * a.p.v_hs;
@@ -556,39 +557,30 @@ __global__ __launch_bounds__(NW * 64, (occ<T, DP, BIAS, NW, true>())) void dq_ke
   const int64_t tok0 = t.q0 + t.pos0, rid0 = tok0 * a.p.Hq + t.head0;
   const int rofs = dpos * a.p.Hq + head - t.head0;
   const int64_t rid = rid0 + rofs;
-  typename Ty<T>::Frag qf[L::NCH], gf[L::NCH], of[L::NCH];
+  typename Ty<T>::Frag qf[L::NCH], gf[L::NCH];
   load_frags<T, DP>(qf, reinterpret_cast<const T*>(a.p.q) + tok0 * a.p.q_ts + t.head0 * a.p.q_hs,
                     valid ? (uint32_t)((dpos * a.p.q_ts + (head - t.head0) * a.p.q_hs) * (int)sizeof(T)) : NO_ROW, D, h);
   load_frags<T, DP>(gf, reinterpret_cast<const T*>(a.p.dout) + tok0 * a.p.do_ts + t.head0 * a.p.do_hs,
                     valid ? (uint32_t)((dpos * a.p.do_ts + (head - t.head0) * a.p.do_hs) * (int)sizeof(T)) : NO_ROW, D, h);
-  load_frags<T, DP>(of, reinterpret_cast<const T*>(a.p.o) + rid0 * D, valid ? (uint32_t)(rofs * D * (int)sizeof(T)) : NO_ROW, D, h);
   const float lse_in = load_f32(a.p.lse + rid0, valid ? 4u * rofs : NO_ROW);
+  const float delta = load_f32(a.delta + rid0, valid ? 4u * rofs : NO_ROW);
   if (BIAS) load_bias<T, NT>(a, lut, t.head0);
   if (sums) {
     for (int i = lane; i < span_of(R); i += 64) hist[i] = 0.f;
     for (int i = lane; i < SKEW; i += 64) skew[i] = 0.f;
   }
   const float lse = valid ? lse_in : INF;
-  float delta = 0.f, big = 0.f;
-#pragma unroll
-  for (int k = 0; k < L::NCH; ++k)
-#pragma unroll
-    for (int e = 0; e < L::EPC; ++e) {
-      delta = fmaf((float)gf[k][e], (float)of[k][e], delta);
-      if (HALF) big = fmaxf(big, fabsf((float)gf[k][e]));
-    }
-  delta = xsum32(delta);
   float up = 1.f;                                              // 1 / (the factor on dS)
   if (HALF) {
+    float big = 0.f;
+#pragma unroll
+    for (int k = 0; k < L::NCH; ++k)
+#pragma unroll
+      for (int e = 0; e < L::EPC; ++e) big = fmaxf(big, fabsf((float)gf[k][e]));
     big = xmax32(big);
     up = 8.f * pow2_of(__float_as_uint(big));
-    if (blockIdx.y == 0) {                                     // for dK / dV: one factor per key head
-      const float wbig = wave_max(big);
-      if (lane == 0 && wbig > 0.f) atomicMax(a.domax + t.kvh, __float_as_uint(wbig));   // order-free
-    }
   }
   const float down = 1.f / up;
-  if (valid && h == 0 && blockIdx.y == 0) a.delta[rid] = delta;
   // dP starts from -delta where the registers allow a copy of it (one subtraction less per score)
   constexpr bool FROM = DP <= 64;
   f16v minus;
@@ -692,7 +684,7 @@ __global__ __launch_bounds__(NW * 64, (occ<T, DP, BIAS, NW, true>())) void dq_ke
       hist[2 * R + MARGIN] = far_hi;                           // (R >= 1: not the same place)
     }
     __syncthreads();
-    float* out = a.hist + ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * NH;
+    float* out = a.hist + ((int64_t)part_no * a.wgs_q + wg) * NH;
     for (int i = threadIdx.x; i < NH; i += NT) {
       float x = 0.f;
 #pragma unroll
@@ -702,8 +694,8 @@ __global__ __launch_bounds__(NW * 64, (occ<T, DP, BIAS, NW, true>())) void dq_ke
   }
   if (!valid) return;
   const float f = a.p.scale * up;
-  if (a.nsplit == 1) store_col(reinterpret_cast<T*>(a.p.dq) + rid * D, o, f, D, h);
-  else store_col(a.part + ((int64_t)blockIdx.y * a.p.total_q * a.p.Hq + rid) * D, o, f, D, h);
+  if (nsplit == 1) store_col(reinterpret_cast<T*>(a.p.dq) + rid * D, o, f, D, h);
+  else store_col(a.part + ((int64_t)part_no * a.p.total_q * a.p.Hq + rid) * D, o, f, D, h);
 }
 
 // sums by relative position of the n workgroups of a head (workgroup i * Hq + head), 16 slices of
@@ -727,15 +719,16 @@ __global__ __launch_bounds__(1024) void hist_bucket_kernel(const float* rel, con
 // backward: dK, dV
 // -------------------------------------------------------------------------------------------
 template <class T, int DP, bool BIAS, int NW>
-__global__ __launch_bounds__(NW * 64, (occ_kv<T, DP, NW>())) void dkv_kernel(Args a) {
+__device__ __forceinline__ void dkv_body(const Args& a, int wg, int part_no) {
   using L = Tile<T, DP>;
   constexpr int NT = NW * 64, BQ = row_tile<T, DP>(), NB = BQ / 32, TILE = BQ * L::RB;
   constexpr bool VL = v_in_lds<T, DP>(), HALF = __is_same(T, _Float16);
   extern __shared__ __attribute__((aligned(16))) char smem[];
+  const int nsplit = a.split_k;
   float* stat = reinterpret_cast<float*>(smem + 4 * TILE);     // [2][lse BQ | -delta BQ]
   float* lut = stat + 4 * BQ;
   char* vt = smem + 4 * TILE + 16 * BQ + (BIAS ? (span_of(a.p.max_distance) * 4 + 15) / 16 * 16 : 0);   // this tile's V (VL)
-  const int kvh = blockIdx.x % a.p.Hkv, tile = blockIdx.x / a.p.Hkv, D = a.p.D, R = a.p.max_distance;
+  const int kvh = wg % a.p.Hkv, tile = wg / a.p.Hkv, D = a.p.D, R = a.p.max_distance;
   const int32_t* tl = a.p.k_tiles + 8 * (int64_t)tile;
   const int64_t q0 = uni(tl[0]), k0 = uni(tl[1]);
   const int nq = uni(tl[2]), nk = uni(tl[3]), key0 = uni(tl[4]), off = nk - nq;
@@ -760,7 +753,7 @@ __global__ __launch_bounds__(NW * 64, (occ_kv<T, DP, NW>())) void dkv_kernel(Arg
 #pragma unroll
   for (int i = 0; i < L::DT; ++i) dk[i] = dv[i] = f16v{};
   float up = 1.f;
-  if (HALF) up = 8.f * pow2_of(a.domax[kvh]);
+  if (HALF) up = 8.f * pow2_of(__float_as_uint(a.domax[kvh]));
   const float down = 1.f / up;
 
   // rows (position * PK + head) that see any of the tile's keys, tile by tile, one head group after
@@ -769,7 +762,7 @@ __global__ __launch_bounds__(NW * 64, (occ_kv<T, DP, NW>())) void dkv_kernel(Arg
   const int lg = a.pk_log, pk = 1 << lg, bp = BQ >> lg, nrows = nq << lg;
   const int first = a.p.causal ? min(max(key0 - off, 0), nq) / bp : 0;
   const int ntq = max((nq + bp - 1) / bp - first, 0), total = a.nsubk * ntq;
-  const int per = (total + a.nsplit - 1) / a.nsplit, t0 = blockIdx.y * per, t1 = min(total, t0 + per);
+  const int t0 = part_no * a.per_k, t1 = min(total, t0 + a.per_k);
   // the first row that sees this lane's key / the wave's first and last key
   const int see = a.p.causal ? (key - off) * pk : 0;
   const int wfirst = a.p.causal ? (key0 + w * 32 - off) * pk : 0;
@@ -895,20 +888,75 @@ __global__ __launch_bounds__(NW * 64, (occ_kv<T, DP, NW>())) void dkv_kernel(Arg
   }
   if (!valid) return;
   const int64_t rid = (k0 + key) * a.p.Hkv + kvh, rows = a.p.total_k * a.p.Hkv;
-  if (a.nsplit == 1) {
+  if (nsplit == 1) {
     store_col(reinterpret_cast<T*>(a.p.dk) + rid * D, dk, a.p.scale * up, D, h);
     store_col(reinterpret_cast<T*>(a.p.dv) + rid * D, dv, 1.f, D, h);
   } else {
-    store_col(a.part + ((int64_t)blockIdx.y * rows + rid) * D, dk, a.p.scale * up, D, h);
-    store_col(a.part + ((int64_t)(a.nsplit + blockIdx.y) * rows + rid) * D, dv, 1.f, D, h);
+    store_col(a.part_k + ((int64_t)part_no * rows + rid) * D, dk, a.p.scale * up, D, h);
+    store_col(a.part_k + ((int64_t)(nsplit + part_no) * rows + rid) * D, dv, 1.f, D, h);
+  }
+}
+
+// -------------------------------------------------------------------------------------------
+// backward: both in one launch.  They need nothing of each other but rowsum(dO O) and max |dO|, which
+// delta_kernel takes first, and share the chip to the end instead of each leaving it half empty: XXX
+// -------------------------------------------------------------------------------------------
+template <class T, int DP, bool BIAS, int NW>
+__global__ __launch_bounds__(NW * 64, (occ_bwd<T, DP, BIAS, NW>())) void bwd_kernel(Args a) {
+  const int id = blockIdx.x, nk = a.wgs_k * a.split_k;
+  if (id < nk) dkv_body<T, DP, BIAS, NW>(a, id % a.wgs_k, id / a.wgs_k);
+  else dq_body<T, DP, BIAS, NW>(a, (id - nk) % a.wgs_q, (id - nk) / a.wgs_q);
+}
+
+// delta[row] = sum dO O over the features, 16 lanes a row, 64 tokens of one head a workgroup; fp16: each
+// workgroup's max |dO| too, of which max_kernel takes a key head's.  (Straight into domax by atomics:
+// 45 us for 1300 workgroups and 12 heads, one cache line.)
+template <class T> __global__ __launch_bounds__(256) void delta_kernel(Args a) {
+  constexpr int EPC = 16 / sizeof(T);
+  constexpr bool HALF = __is_same(T, _Float16);
+  const int head = blockIdx.y, l = threadIdx.x & 15, D = a.p.D;
+  float big = 0.f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int64_t tok = (int64_t)blockIdx.x * 64 + i * 16 + (threadIdx.x >> 4);
+    float x = 0.f;
+    if (tok < a.p.total_q) {
+      const T* g = reinterpret_cast<const T*>(a.p.dout) + tok * a.p.do_ts + head * a.p.do_hs;
+      const T* o = reinterpret_cast<const T*>(a.p.o) + (tok * a.p.Hq + head) * D;
+#pragma unroll
+      for (int j = 0; j < 128 / (16 * EPC); ++j) {
+        const int d = (16 * j + l) * EPC;
+        if (d >= D) continue;
+        const auto gv = *reinterpret_cast<const typename Ty<T>::Frag*>(g + d);
+        const auto ov = *reinterpret_cast<const typename Ty<T>::Frag*>(o + d);
+#pragma unroll
+        for (int e = 0; e < EPC; ++e) {
+          x = fmaf((float)gv[e], (float)ov[e], x);
+          if (HALF) big = fmaxf(big, fabsf((float)gv[e]));
+        }
+      }
+    }
+    x += dpp_mov<0x128>(x);                                    // over the row's 16 lanes
+    x += dpp_mov<0x124>(x);
+    x += dpp_mov<0x4e>(x);
+    x += dpp_mov<0xb1>(x);
+    if (tok < a.p.total_q && l == 0) a.delta[tok * a.p.Hq + head] = x;
+  }
+  if (HALF) {
+    __shared__ float waves[4];
+    big = wave_max(big);
+    if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = big;
+    __syncthreads();
+    if (threadIdx.x == 0)
+      a.wgmax[(int64_t)head * gridDim.x + blockIdx.x] = fmaxf(fmaxf(waves[0], waves[1]), fmaxf(waves[2], waves[3]));
   }
 }
 
 // ---- host: one launcher per type (packed_attention_<type>.hip) ------------------------------
 struct Plan {
   Args a;
-  int dp, nwq, nwk, split_q, split_k;
-  int64_t part_bytes, delta_bytes, hist_bytes, rel_bytes, dom_bytes;   // carved in this order
+  int dp, nwq, nwk;            // waves of a workgroup over queries, over keys (backward: the same)
+  int64_t hist_bytes;
 };
 template <class T> int run_fwd(const Plan& p, hipStream_t s);
 template <class T> int run_bwd(const Plan& p, hipStream_t s);
@@ -925,67 +973,65 @@ template <class T, class K> int launch(K kernel, dim3 grid, int threads, size_t 
 }
 
 template <class T, int DP, bool BIAS> int fwd_dp(const Plan& p, hipStream_t s) {
-  Args a = p.a;
-  a.nsplit = p.split_q;
-  const int wgs = a.p.n_q_tiles * a.p.Hkv * a.nsub;
+  const Args& a = p.a;
   const size_t lds = 4 * key_tile<T, DP>() * Tile<T, DP>::RB + (BIAS ? span_of(a.p.max_distance) * 4 : 0);
-  const int rc = p.nwq == 2 ? launch<T>(fwd_kernel<T, DP, BIAS, 2>, dim3(wgs, a.nsplit), 128, lds, a, s)
-                            : launch<T>(fwd_kernel<T, DP, BIAS, 4>, dim3(wgs, a.nsplit), 256, lds, a, s);
-  if (rc || a.nsplit == 1) return rc;
+  const int rc = p.nwq == 2 ? launch<T>(fwd_kernel<T, DP, BIAS, 2>, dim3(a.wgs_q, a.split_q), 128, lds, a, s)
+                            : launch<T>(fwd_kernel<T, DP, BIAS, 4>, dim3(a.wgs_q, a.split_q), 256, lds, a, s);
+  if (rc || a.split_q == 1) return rc;
   const int64_t rows = a.p.total_q * a.p.Hq;
-  hipLaunchKernelGGL((join_kernel<T, true>), dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, s, a.part, a.part_lse, a.nsplit,
+  hipLaunchKernelGGL((join_kernel<T, true>), dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, s, a.part, a.part_lse, a.split_q,
                      rows, a.p.D, reinterpret_cast<T*>(a.p.o), nullptr, a.p.lse);
   VAESNE_CHECK_LAUNCH();
   return 0;
 }
 
-__global__ __launch_bounds__(64) void clear_kernel(uint32_t* p, int n);
+// domax[head] = max of the n values of the head's group (0 for none)
+__global__ __launch_bounds__(256) void max_kernel(const float* wgmax, int64_t n, float* domax);
 
 template <class T, int DP, bool BIAS> int bwd_dp(const Plan& p, hipStream_t s) {
-  Args a = p.a;
-  const int NH = 2 * a.p.max_distance + 1;
-  constexpr int BN = key_tile<T, DP>(), RB = Tile<T, DP>::RB;
-  if (__is_same(T, _Float16)) {
-    hipLaunchKernelGGL(clear_kernel, dim3((a.p.Hkv + 63) / 64), dim3(64), 0, s, a.domax, a.p.Hkv);
+  const Args& a = p.a;
+  constexpr int BN = key_tile<T, DP>(), BQ = row_tile<T, DP>(), RB = Tile<T, DP>::RB;
+  const int R = a.p.max_distance, NH = 2 * R + 1, nw = p.nwq;
+  const int64_t blocks = (a.p.total_q + 63) / 64;
+  if (blocks > 0) {
+    hipLaunchKernelGGL((delta_kernel<T>), dim3((unsigned)blocks, a.p.Hq), dim3(256), 0, s, a);
     VAESNE_CHECK_LAUNCH();
   }
-  if (a.p.n_q_tiles > 0) {
-    a.nsplit = p.split_q;
-    const int wgs = a.p.n_q_tiles * a.p.Hkv * a.nsub;
-    const size_t lds = 4 * BN * RB + (BIAS ? ((1 + p.nwq) * span_of(a.p.max_distance) + 3) / 4 * 16 : 0) +
-                       (BIAS && a.p.dtable ? p.nwq * SKEW * 4 : 0);
-    const int rc = p.nwq == 2 ? launch<T>(dq_kernel<T, DP, BIAS, 2>, dim3(wgs, a.nsplit), 128, lds, a, s)
-                              : launch<T>(dq_kernel<T, DP, BIAS, 4>, dim3(wgs, a.nsplit), 256, lds, a, s);
+  if (__is_same(T, _Float16)) {
+    hipLaunchKernelGGL(max_kernel, dim3(a.p.Hkv), dim3(256), 0, s, a.wgmax, blocks * a.group, a.domax);
+    VAESNE_CHECK_LAUNCH();
+  }
+  const size_t lds_q = 4 * BN * RB + (BIAS ? ((1 + nw) * span_of(R) + 3) / 4 * 16 : 0) + (BIAS && a.p.dtable ? nw * SKEW * 4 : 0);
+  const size_t lds_k = 4 * BQ * RB + 16 * BQ + (BIAS ? (span_of(R) * 4 + 15) / 16 * 16 : 0) +
+                       (v_in_lds<T, DP>() ? nw * 32 * RB : 0);
+  const size_t lds = lds_q > lds_k ? lds_q : lds_k;
+  const int wgs = a.wgs_k * a.split_k + a.wgs_q * a.split_q;
+  if (wgs > 0) {
+    const int rc = nw == 2 ? launch<T>(bwd_kernel<T, DP, BIAS, 2>, dim3(wgs), 128, lds, a, s)
+                           : launch<T>(bwd_kernel<T, DP, BIAS, 4>, dim3(wgs), 256, lds, a, s);
     if (rc) return rc;
-    if (a.nsplit > 1) {
-      const int64_t rows = a.p.total_q * a.p.Hq;
-      hipLaunchKernelGGL((join_kernel<T, false>), dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, s, a.part, nullptr,
-                         a.nsplit, rows, a.p.D, reinterpret_cast<T*>(a.p.dq), nullptr, nullptr);
-      VAESNE_CHECK_LAUNCH();
-    }
+  }
+  if (a.split_q > 1) {
+    const int64_t rows = a.p.total_q * a.p.Hq;
+    hipLaunchKernelGGL((join_kernel<T, false>), dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, s, a.part, nullptr, a.split_q,
+                       rows, a.p.D, reinterpret_cast<T*>(a.p.dq), nullptr, nullptr);
+    VAESNE_CHECK_LAUNCH();
+  }
+  if (a.split_k > 1) {
+    const int64_t rows = a.p.total_k * a.p.Hkv;
+    hipLaunchKernelGGL((join_kernel<T, false>), dim3((unsigned)((rows + 7) / 8), 2), dim3(256), 0, s, a.part_k, nullptr,
+                       a.split_k, rows, a.p.D, reinterpret_cast<T*>(a.p.dk), reinterpret_cast<T*>(a.p.dv), nullptr);
+    VAESNE_CHECK_LAUNCH();
   }
   if (BIAS && a.p.dtable) {
     float* rel = a.hist + p.hist_bytes / 4;
-    hipLaunchKernelGGL(hist_sum_kernel, dim3((NH + 63) / 64, a.p.Hq), dim3(1024), 0, s, a.hist,
-                       a.p.n_q_tiles * p.split_q, a.p.Hq, NH, rel);
+    hipLaunchKernelGGL(hist_sum_kernel, dim3((NH + 63) / 64, a.p.Hq), dim3(1024), 0, s, a.hist, a.p.n_q_tiles * a.split_q,
+                       a.p.Hq, NH, rel);
     VAESNE_CHECK_LAUNCH();
     hipLaunchKernelGGL((hist_bucket_kernel<T>), dim3(a.p.Hq), dim3(1024), 0, s, rel, a.p.lut, NH, a.p.Hq,
                        a.p.num_buckets, reinterpret_cast<T*>(a.p.dtable));
     VAESNE_CHECK_LAUNCH();
   }
-  if (a.p.n_k_tiles == 0) return 0;
-  a.nsplit = p.split_k;
-  constexpr int BQ = row_tile<T, DP>();
-  const size_t lds = 4 * BQ * RB + 16 * BQ + (BIAS ? (span_of(a.p.max_distance) * 4 + 15) / 16 * 16 : 0) +
-                     (v_in_lds<T, DP>() ? p.nwk * 32 * RB : 0);
-  const int wgs = a.p.n_k_tiles * a.p.Hkv;
-  const int rc = p.nwk == 2 ? launch<T>(dkv_kernel<T, DP, BIAS, 2>, dim3(wgs, a.nsplit), 128, lds, a, s)
-                            : launch<T>(dkv_kernel<T, DP, BIAS, 4>, dim3(wgs, a.nsplit), 256, lds, a, s);
-  if (rc || a.nsplit == 1) return rc;
-  const int64_t rows = a.p.total_k * a.p.Hkv;
-  hipLaunchKernelGGL((join_kernel<T, false>), dim3((unsigned)((rows + 7) / 8), 2), dim3(256), 0, s, a.part, nullptr, a.nsplit,
-                     rows, a.p.D, reinterpret_cast<T*>(a.p.dk), reinterpret_cast<T*>(a.p.dv), nullptr);
-  VAESNE_CHECK_LAUNCH();
   return 0;
 }
 

@@ -17,9 +17,14 @@ template <> int run_bwd<float>(const Plan& p, hipStream_t s);
 template <> int run_bwd<__bf16>(const Plan& p, hipStream_t s);
 template <> int run_bwd<_Float16>(const Plan& p, hipStream_t s);
 
-__global__ __launch_bounds__(64) void clear_kernel(uint32_t* p, int n) {
-  const int i = blockIdx.x * 64 + threadIdx.x;
-  if (i < n) p[i] = 0;
+__global__ __launch_bounds__(256) void max_kernel(const float* wgmax, int64_t n, float* domax) {
+  __shared__ float waves[4];
+  float x = 0.f;
+  for (int64_t i = threadIdx.x; i < n; i += 256) x = fmaxf(x, wgmax[blockIdx.x * n + i]);
+  x = wave_max(x);
+  if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = x;
+  __syncthreads();
+  if (threadIdx.x == 0) domax[blockIdx.x] = fmaxf(fmaxf(waves[0], waves[1]), fmaxf(waves[2], waves[3]));
 }
 
 __global__ __launch_bounds__(1024) void hist_sum_kernel(const float* hist, int n, int Hq, int NH, float* rel) {
@@ -45,24 +50,28 @@ constexpr int64_t MAX_PART = 256 << 20;
 constexpr int64_t MAX_STRIDE = 1 << 21;  // elements: a tile of 128 rows spans less than 2^31 bytes
 constexpr int64_t MAX_ROWS = 1 << 25; // rows of one sequence: 32-bit row arithmetic with room
 
-// Parts to cut the streamed axis into.  Each of `wgs` workgroups walks up to `longest` tiles, `mean` on
-// average; `slots` of them run at once, longest first.  A part costs about six tiles more (its own
-// loads, its sums to memory and their joining), so the end of the launch is estimated as
-//   (all tiles and parts) / slots + half of the longest part, at least the longest part,
-// eight tiles more for the joining launch, and the cheapest count of parts of 4 tiles or more taken.  (fp16 training, 6 sequences of up to 2047, 12 heads: one part 48 us
-// forward, two 58 + 17 us; dK / dV of the bf16 training step: one part 873 us, two 680 + 22 us.)
-int splits(int64_t wgs, int64_t longest, double mean, int64_t part_bytes, int slots) {
-  const double over = 6, join = 8;
+// Parts to cut the streamed axis into, in units of a tile (about 1.2 us).  Each of `wgs` workgroups walks
+// up to `longest` tiles, `mean` on average; SLOTS of them run at once, longest first, beside `beside`
+// units of other work.  Parts have the same length for all (a shorter walk has fewer of them), cost about
+// six tiles more each, and are written and read back once (4.5 TB/s) by a joining launch.  The end of the launch is estimated as
+//   max(all tiles and parts / SLOTS + beside + half of the longest part, the longest part) + joining
+// and the fewest parts taken that come within a twentieth of the best.  (fp16 training, 6 sequences of up
+// to 2047, 12 heads: one part 48 us forward, two 58 + 17 us; one token over 32 caches of up to 16384
+// keys: one part 0.35 ms, as chosen 0.13.)
+int splits(int64_t wgs, int64_t longest, double mean, int64_t part_bytes, double beside) {
+  const double over = 6;
   const int64_t most = std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(MAX_SPLIT, longest / 4),
                                                               MAX_PART / std::max<int64_t>(part_bytes, 1)));
   auto end = [&](int64_t n) {
     const double own = (double)((longest + n - 1) / n) + over;
-    return std::max(wgs * (mean + n * over) / slots + 0.5 * own, own) + (n > 1 ? join : 0);
+    const double join = n > 1 ? 4 + (double)n * part_bytes / 2.7e6 : 0;
+    const double parts = std::max(1.0, n * mean / std::max<double>(longest, 1));
+    return std::max(wgs * (mean + parts * over) / SLOTS + beside + 0.5 * own, own) + join;
   };
   double least = end(1);
   for (int64_t n = 2; n <= most; ++n) least = std::min(least, end(n));
   for (int64_t n = 1; n < most; ++n)
-    if (end(n) <= 1.05 * least) return (int)n;         // the fewest parts that come within a twentieth
+    if (end(n) <= 1.05 * least) return (int)n;
   return (int)most;
 }
 
@@ -96,54 +105,62 @@ int log_heads_per_row_tile(const vaesne_packed_attn* a, int dp, int waves) {
 
 int waves_for(int64_t rows) { return rows <= 64 ? 2 : 4; }
 
-int make_plan(const vaesne_packed_attn* a, Plan* p) {
+int make_plan(const vaesne_packed_attn* a, int backward, Plan* p) {
   if (!sizes_ok(a)) return (int)hipErrorInvalidValue;
   *p = Plan{};
-  p->a.p = *a;
-  p->a.group = a->Hq / a->Hkv;
-  p->a.pg = heads_per_tile(a);
-  p->a.nsub = p->a.group / p->a.pg;
-  p->a.pgm = p->a.pg == 1 ? 0u : (uint32_t)(((1ull << 32) + p->a.pg - 1) / p->a.pg);
-  if ((int64_t)a->max_q * p->a.pg > MAX_ROWS || (int64_t)a->max_k * p->a.pg > MAX_ROWS) return (int)hipErrorInvalidValue;
-  p->a.c = a->scale * LOG2E;
+  Args& r = p->a;
+  r.p = *a;
+  r.group = a->Hq / a->Hkv;
+  r.pg = heads_per_tile(a);
+  r.nsub = r.group / r.pg;
+  r.pgm = r.pg == 1 ? 0u : (uint32_t)(((1ull << 32) + r.pg - 1) / r.pg);
+  if ((int64_t)a->max_q * r.pg > MAX_ROWS || (int64_t)a->max_k * r.pg > MAX_ROWS) return (int)hipErrorInvalidValue;
+  r.c = a->scale * LOG2E;
   p->dp = a->D <= 16 ? 16 : a->D <= 32 ? 32 : a->D <= 64 ? 64 : 128;
-  p->nwq = waves_for((int64_t)a->max_q * p->a.pg);
-  p->nwk = waves_for(a->max_k);
-  p->a.pk_log = log_heads_per_row_tile(a, p->dp, p->nwk);
-  p->a.nsubk = p->a.group >> p->a.pk_log;
+  const int64_t rows = (int64_t)a->max_q * r.pg;
+  p->nwk = waves_for(std::max<int64_t>(rows, a->max_k));
+  p->nwq = backward ? p->nwk : waves_for(rows);
+  r.pk_log = log_heads_per_row_tile(a, p->dp, p->nwk);
+  r.nsubk = r.group >> r.pk_log;
   const int bn = a->type == 0 ? 32 : 64;
   const int64_t qrows = a->total_q * a->Hq, krows = a->total_k * a->Hkv;
   const double n = std::max(a->nseq, 1);
-  p->split_q = splits((int64_t)a->n_q_tiles * a->Hkv * p->a.nsub, (a->max_k + bn - 1) / bn, a->total_k / n / bn,
-                      qrows * (a->D + 1) * 4, SLOTS);
-  const int bp = (a->type != 0 && p->dp == 128 ? 32 : bn) >> p->a.pk_log;   // row_tile()
-  p->split_k = splits((int64_t)a->n_k_tiles * a->Hkv, (int64_t)p->a.nsubk * ((a->max_q + bp - 1) / bp),
-                      (double)p->a.nsubk * a->total_q / n / bp, 2 * krows * a->D * 4, SLOTS);
+  r.wgs_q = a->n_q_tiles * a->Hkv * r.nsub;
+  r.wgs_k = backward ? a->n_k_tiles * a->Hkv : 0;
+  const int bp = (a->type != 0 && p->dp == 128 ? 32 : bn) >> r.pk_log;   // row_tile()
+  const double mean_q = a->total_k / n / bn, mean_k = (double)r.nsubk * a->total_q / n / bp;
+  const int64_t long_q = (a->max_k + bn - 1) / bn, long_k = (int64_t)r.nsubk * ((a->max_q + bp - 1) / bp);
+  r.split_q = splits(r.wgs_q, long_q, mean_q, qrows * (a->D + 1) * 4, r.wgs_k * mean_k / SLOTS);
+  r.split_k = splits(r.wgs_k, long_k, mean_k, 2 * krows * a->D * 4, r.wgs_q * mean_q / SLOTS);
+  r.per_q = (int)((long_q + r.split_q - 1) / r.split_q);
+  r.per_k = (int)((long_k + r.split_k - 1) / r.split_k);
   return 0;
 }
 
-// the workspace: split parts, their statistics | rowsum(dO O) | bias sums | max |dO|
+// the workspace: parts of the forward or dQ, their statistics | of dK / dV | rowsum(dO O) | bias sums |
+// max |dO|
 int64_t carve(Plan* p, int backward) {
-  const vaesne_packed_attn& a = p->a.p;
+  Args& r = p->a;
+  const vaesne_packed_attn& a = r.p;
   const int64_t qrows = a.total_q * a.Hq, krows = a.total_k * a.Hkv, NH = 2 * a.max_distance + 1;
-  int64_t part = 0;
-  if (p->split_q > 1) part = p->split_q * qrows * a.D * 4;
-  if (backward && p->split_k > 1) part = std::max(part, 2 * p->split_k * krows * a.D * 4);
-  p->part_bytes = up16(part);
-  const int64_t lse = !backward && p->split_q > 1 ? up16(p->split_q * qrows * 4) : 0;
-  p->delta_bytes = backward ? up16(qrows * 4) : 0;
   const bool bias = backward && a.table && a.dtable;
-  p->hist_bytes = bias ? up16((int64_t)a.n_q_tiles * a.Hq * p->split_q * NH * 4) : 0;
-  p->rel_bytes = bias ? up16((int64_t)a.Hq * NH * 4) : 0;
-  p->dom_bytes = backward && a.type == 2 ? up16((int64_t)a.Hkv * 4) : 0;
-  char* w = reinterpret_cast<char*>(a.workspace);
-  p->a.part = reinterpret_cast<float*>(w);
-  p->a.part_lse = reinterpret_cast<float*>(w + p->part_bytes);
-  w += p->part_bytes + lse;
-  p->a.delta = reinterpret_cast<float*>(w);
-  p->a.hist = reinterpret_cast<float*>(w + p->delta_bytes);
-  p->a.domax = reinterpret_cast<uint32_t*>(w + p->delta_bytes + p->hist_bytes + p->rel_bytes);
-  return p->part_bytes + lse + p->delta_bytes + p->hist_bytes + p->rel_bytes + p->dom_bytes;
+  p->hist_bytes = bias ? up16((int64_t)a.n_q_tiles * a.Hq * r.split_q * NH * 4) : 0;
+  int64_t used = 0;
+  auto take = [&](int64_t bytes) {
+    float* at = reinterpret_cast<float*>(reinterpret_cast<uintptr_t>(a.workspace) + used);
+    used += up16(bytes);
+    return at;
+  };
+  r.part = take(r.split_q > 1 ? r.split_q * qrows * a.D * 4 : 0);
+  r.part_lse = take(!backward && r.split_q > 1 ? r.split_q * qrows * 4 : 0);
+  r.part_k = take(backward && r.split_k > 1 ? 2 * r.split_k * krows * a.D * 4 : 0);
+  r.delta = take(backward ? qrows * 4 : 0);
+  r.hist = take(p->hist_bytes);
+  take(bias ? (int64_t)a.Hq * NH * 4 : 0);                       // behind hist: its sums
+  const bool half = backward && a.type == 2;
+  r.domax = take(half ? (int64_t)a.Hkv * 4 : 0);
+  r.wgmax = take(half ? (a.total_q + 63) / 64 * a.Hq * 4 : 0);
+  return used;
 }
 
 bool aligned(const void* p, int64_t ts, int64_t hs, int size) {
@@ -155,7 +172,7 @@ int check(const Plan& p, int64_t bytes, int backward) {
   const vaesne_packed_attn& a = p.a.p;
   const int size = a.type == 0 ? 4 : 2;
   const int bad = (int)hipErrorInvalidValue;
-  if (a.q_tile != p.nwq * 32 / p.a.pg || a.k_tile != p.nwk * 32) return bad;
+  if (a.q_tile != p.nwq * 32 / p.a.pg || (backward && a.k_tile != p.nwk * 32)) return bad;
   if (a.n_q_tiles < 0 || a.n_k_tiles < 0 || (a.total_q > 0 && (a.n_q_tiles == 0 || !a.q_tiles || !a.q || !a.o || !a.lse)) ||
       (a.total_k > 0 && (!a.k || !a.v)))
     return bad;
@@ -179,9 +196,9 @@ int check(const Plan& p, int64_t bytes, int backward) {
 }  // namespace pk
 }  // namespace vaesne
 
-VAESNE_API int vaesne_packed_attn_tiles(const vaesne_packed_attn* a, int* q_tile, int* k_tile) {
+VAESNE_API int vaesne_packed_attn_tiles(const vaesne_packed_attn* a, int backward, int* q_tile, int* k_tile) {
   Plan p;
-  const int rc = make_plan(a, &p);
+  const int rc = make_plan(a, backward, &p);
   if (rc) return rc;
   *q_tile = p.nwq * 32 / p.a.pg;
   *k_tile = p.nwk * 32;
@@ -190,13 +207,13 @@ VAESNE_API int vaesne_packed_attn_tiles(const vaesne_packed_attn* a, int* q_tile
 
 VAESNE_API int64_t vaesne_packed_attn_workspace(const vaesne_packed_attn* a, int backward) {
   Plan p;
-  if (make_plan(a, &p)) return -1;
+  if (make_plan(a, backward, &p)) return -1;
   return carve(&p, backward);
 }
 
 VAESNE_API int vaesne_packed_attn_fwd(const vaesne_packed_attn* a, void* stream) {
   Plan p;
-  int rc = make_plan(a, &p);
+  int rc = make_plan(a, 0, &p);
   if (!rc) rc = check(p, carve(&p, 0), 0);
   if (rc || a->total_q == 0) return rc;
   hipStream_t s = (hipStream_t)stream;
@@ -205,7 +222,7 @@ VAESNE_API int vaesne_packed_attn_fwd(const vaesne_packed_attn* a, void* stream)
 
 VAESNE_API int vaesne_packed_attn_bwd(const vaesne_packed_attn* a, void* stream) {
   Plan p;
-  int rc = make_plan(a, &p);
+  int rc = make_plan(a, 1, &p);
   if (!rc) rc = check(p, carve(&p, 1), 1);
   if (rc) return rc;
   hipStream_t s = (hipStream_t)stream;
