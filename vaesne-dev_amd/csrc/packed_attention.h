@@ -296,7 +296,7 @@ struct QTile {
 
 // scores of one 32x32 tile to the log2 domain with bias, s c + bias + more.  Register r's relative position is
 // rel0 + SIGN acc_row(r, h); lo .. hi (uniform) bounds those of the tile.
-template <int SIGN>
+template <int SIGN, bool MORE>
 __device__ __forceinline__ void add_bias(f16v& s, float c, const float* lut, int rel0, int lo, int hi, int h, int R,
                                          float more = 0.f) {
   if (hi <= -R || lo >= R) {                               // one bucket for the whole tile
@@ -306,32 +306,33 @@ __device__ __forceinline__ void add_bias(f16v& s, float c, const float* lut, int
   } else {
     const float* p = lut + (rel0 + SIGN * 4 * h + R + MARGIN);
 #pragma unroll
-    for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], c, p[SIGN * acc_row(r, 0)] + more);
+    for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], c, MORE ? p[SIGN * acc_row(r, 0)] + more : p[SIGN * acc_row(r, 0)]);
   }
 }
 
 // -------------------------------------------------------------------------------------------
 // forward
 // -------------------------------------------------------------------------------------------
-template <class T, int DP> constexpr int key_tile() { return sizeof(T) == 2 ? 64 : 32; }
+// keys of a tile.  32 in two-wave workgroups at head_dim 128: few rows are bound by the reads of K and V, and
+// 32 KB of LDS let four of them run on a CU (one token over 32 caches of up to 16384 keys, 0.43 GB: 64 keys 124 us, 32 96 us).
+template <class T, int DP, int NW> constexpr int key_tile() { return sizeof(T) == 4 || (DP == 128 && NW == 2) ? 32 : 64; }
 // dK / dV at head_dim 128 hold 128 registers of sums: V goes to LDS and the row tile is 32, so that two
 // waves per SIMD fit (causal training step of 10 k tokens, 16 heads over 4: V in registers at one
 // wave 0.59 ms, at two, spilling, 1.50 ms; so 0.50 ms)
 template <class T, int DP> constexpr bool v_in_lds() { return sizeof(T) == 2 && DP == 128; }
 // waves per SIMD the registers are budgeted for.  One (all 512 registers) where two would spill: fp32 at
-// wide heads, and two-wave workgroups at head_dim 128, which stage twice as much per thread (their LDS
-// allows one wave per SIMD anyway).
-template <class T, int DP, int NW> constexpr int occ_fwd() { return DP == 128 && (sizeof(T) == 4 || NW == 2) ? 1 : 2; }
+// wide heads, and in the backward two-wave workgroups and a bias at head_dim 128.
+template <class T, int DP, int NW> constexpr int occ_fwd() { return DP == 128 && sizeof(T) == 4 ? 1 : 2; }
 template <class T, int DP, bool BIAS, int NW> constexpr int occ_bwd() {
   return (sizeof(T) == 4 && DP >= 64) || (DP == 128 && (NW == 2 || BIAS)) ? 1 : 2;
 }
 // query rows of a tile in dK / dV
-template <class T, int DP> constexpr int row_tile() { return v_in_lds<T, DP>() ? 32 : key_tile<T, DP>(); }
+template <class T, int DP> constexpr int row_tile() { return sizeof(T) == 4 || v_in_lds<T, DP>() ? 32 : 64; }
 
 template <class T, int DP, bool BIAS, int NW>
 __global__ __launch_bounds__(NW * 64, (occ_fwd<T, DP, NW>())) void fwd_kernel(Args a) {
   using L = Tile<T, DP>;
-  constexpr int NT = NW * 64, BN = key_tile<T, DP>(), NB = BN / 32, TILE = BN * L::RB;
+  constexpr int NT = NW * 64, BN = key_tile<T, DP, NW>(), NB = BN / 32, TILE = BN * L::RB;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   float* lut = reinterpret_cast<float*>(smem + 4 * TILE);
   const int nh = a.p.Hkv * a.nsub;
@@ -390,12 +391,16 @@ __global__ __launch_bounds__(NW * 64, (occ_fwd<T, DP, NW>())) void fwd_kernel(Ar
         for (int k = 0; k < L::NCH; ++k) s[n] = mma(L::row(K, at, 32 * n, k), qf[k], s[n]);
       }
       feed<NB * L::NCH, 1, 4>();
-      // scores to the units of the running maximum: raw without a bias, log2 with one
-      const float c = BIAS ? 1.f : a.c;
-      if (BIAS) {
+      // to the log2 domain, from the running origin m on: s c [+ bias] - m
+      const float from = m == -INF ? 0.f : -m;
 #pragma unroll
-        for (int n = 0; n < NB; ++n)
-          add_bias<1>(s[n], a.c, lut, base + 32 * n - qabs, base + 32 * n - qfirst - 31, base + 32 * n - qfirst + 31, h, R);
+      for (int n = 0; n < NB; ++n) {
+        if constexpr (BIAS) {
+          add_bias<1, true>(s[n], a.c, lut, base + 32 * n - qabs, base + 32 * n - qfirst - 31, base + 32 * n - qfirst + 31, h, R, from);
+        } else {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) s[n][r] = fmaf(s[n][r], a.c, from);
+        }
       }
       if (base + BN > wmin) {
 #pragma unroll
@@ -410,24 +415,31 @@ __global__ __launch_bounds__(NW * 64, (occ_fwd<T, DP, NW>())) void fwd_kernel(Ar
 #pragma unroll
         for (int r = 0; r < 16; ++r) mt = fmaxf(mt, s[n][r]);
       mt = xmax32(mt);
-      // the origin moves only when a score exceeds it by 2^8: exp2 stays <= 2^8, sums fp32
-      if (__any(mt > m + 8.f / c)) {
-        const float mn = fmaxf(m, mt), f = mn == -INF ? 1.f : __builtin_amdgcn_exp2f((m - mn) * c);
-        m = mn;
+      // the origin moves when the first key is seen, and only when a score exceeds it by 2^8 after that:
+      // exp2 stays <= 2^8, the sums are fp32
+      if (__any(mt > 8.f || (m == -INF && mt > -INF))) {
+        const bool first = m == -INF;
+        const float up = first ? mt : fmaxf(mt, 0.f);             // from the old origin (0 at first)
+        const float f = first ? 0.f : __builtin_amdgcn_exp2f(-up);
+        const float by = up == -INF ? 0.f : up;
+        m = first ? mt : m + up;
         l *= f;
 #pragma unroll
         for (int i = 0; i < L::DT; ++i)
 #pragma unroll
           for (int r = 0; r < 16; ++r) o[i][r] *= f;
+#pragma unroll
+        for (int n = 0; n < NB; ++n)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) s[n][r] -= by;
       }
-      const float mc = m == -INF ? 0.f : -m * c;
 #pragma unroll
-      for (int n = 0; n < NB; ++n)
+      for (int n = 0; n < NB; ++n) {
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          s[n][r] = __builtin_amdgcn_exp2f(fmaf(s[n][r], c, mc));
-          l += s[n][r];
-        }
+        for (int r = 0; r < 16; ++r) s[n][r] = __builtin_amdgcn_exp2f(s[n][r]);
+#pragma unroll
+        for (int r = 0; r < 16; r += 4) l += (s[n][r] + s[n][r + 1]) + (s[n][r + 2] + s[n][r + 3]);
+      }
 #pragma unroll
       for (int n = 0; n < NB; ++n)
 #pragma unroll
@@ -452,7 +464,7 @@ __global__ __launch_bounds__(NW * 64, (occ_fwd<T, DP, NW>())) void fwd_kernel(Ar
   l = xsum32(l);
   if (!valid) return;
   const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);      // (a NaN sum stays one)
-  const float lse = l == 0.f ? INF : fmaf(m, BIAS ? 1.f : a.c, __log2f(l));
+  const float lse = l == 0.f ? INF : m + __log2f(l);
   const int64_t rid = (t.q0 + t.pos0 + dpos) * a.p.Hq + head;
   if (a.split_q == 1) {
     store_col(reinterpret_cast<T*>(a.p.o) + rid * D, o, inv, D, h);
@@ -464,9 +476,10 @@ __global__ __launch_bounds__(NW * 64, (occ_fwd<T, DP, NW>())) void fwd_kernel(Ar
   }
 }
 
-// Joins the parts of `rows` rows of D: weighted by their log-sum-exp (WEIGHTED: the forward; +inf
-// marks a part that saw nothing) or plainly summed, in the order of the parts.  8 rows per
-// workgroup, 32 lanes of 4 columns each.
+// Joins the n <= 64 parts of `rows` rows of D: weighted by their log-sum-exp (WEIGHTED: the forward; +inf
+// marks a part that saw nothing and was not written) or plainly summed, in the order of the parts.  8 rows per
+// workgroup, 32 lanes of 4 columns each; a lane takes the weights of parts l and l + 32, and eight parts
+// are in flight (one after the other: 12 us instead of 5 for 20 parts of 1024 rows).
 template <class T, bool WEIGHTED>
 __global__ __launch_bounds__(256) void join_kernel(const float* part, const float* part_lse, int n, int64_t rows,
                                                    int D, T* out, T* out2, float* lse) {
@@ -474,35 +487,53 @@ __global__ __launch_bounds__(256) void join_kernel(const float* part, const floa
     part += (int64_t)n * rows * D;
     out = out2;
   }
-  const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-  const int d = (threadIdx.x & 31) * 4;
-  if (row >= rows) return;
-  f4 acc = {0.f, 0.f, 0.f, 0.f};
-  float m = -INF, sum = 0.f;
+  const int l = threadIdx.x & 31, d = l * 4;
+  const int64_t row0 = (int64_t)blockIdx.x * 8, row = row0 + (threadIdx.x >> 5);
+  const bool live = row < rows;
+  float w[2] = {l < n ? 1.f : 0.f, l + 32 < n ? 1.f : 0.f};
   if (WEIGHTED) {
-    for (int i = 0; i < n; ++i) {
-      const float x = part_lse[i * rows + row];
-      if (x != INF) m = fmaxf(m, x);
-    }
-    for (int i = 0; i < n; ++i) {
-      const float x = part_lse[i * rows + row];
-      if (x != INF) sum += __builtin_amdgcn_exp2f(x - m);
-    }
-  }
-  if (d < D)
-    for (int i = 0; i < n; ++i) {
-      float wgt = 1.f;
-      if (WEIGHTED) {
-        const float x = part_lse[i * rows + row];
-        if (x == INF) continue;
-        wgt = __builtin_amdgcn_exp2f(x - m) / sum;
-      }
-      const f4 p = *reinterpret_cast<const f4*>(part + (i * rows + row) * D + d);
+    float x[2] = {INF, INF};
 #pragma unroll
-      for (int e = 0; e < 4; ++e) acc[e] = fmaf(wgt, p[e], acc[e]);
+    for (int i = 0; i < 2; ++i)
+      if (live && l + 32 * i < n) x[i] = part_lse[(int64_t)(l + 32 * i) * rows + row];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) if (x[i] == INF) x[i] = -INF;
+    float m = fmaxf(x[0], x[1]);                       // (a NaN is not lost: its weight below is one)
+    m = xmax16(m);
+    m = fmaxf(m, dpp_mov<0x128>(m));
+    m = fmaxf(m, dpp_mov<0x124>(m));
+    m = fmaxf(m, dpp_mov<0x4e>(m));
+    m = fmaxf(m, dpp_mov<0xb1>(m));
+#pragma unroll
+    for (int i = 0; i < 2; ++i) w[i] = x[i] == -INF ? 0.f : __builtin_amdgcn_exp2f(x[i] - m);
+    float sum = w[0] + w[1];
+    sum = xsum16(sum);
+    sum += dpp_mov<0x128>(sum);
+    sum += dpp_mov<0x124>(sum);
+    sum += dpp_mov<0x4e>(sum);
+    sum += dpp_mov<0xb1>(sum);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) w[i] = w[i] == 0.f ? 0.f : w[i] / sum;
+    if (live && l == 0) lse[row] = sum == 0.f ? INF : m + __log2f(sum);
+  }
+  f4 acc = {0.f, 0.f, 0.f, 0.f};
+  const uint32_t at = live && d < D ? (uint32_t)(((threadIdx.x >> 5) * D + d) * 4) : NO_ROW;
+  for (int i0 = 0; i0 < n; i0 += 8) {
+    f4 p[8];
+    float wi[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      wi[i] = __shfl(i0 < 32 ? w[0] : w[1], (i0 + i) & 31, 32);
+      const auto rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(part + ((int64_t)min(i0 + i, n - 1) * rows + row0) * D),
+                                                          0, 0x7fffffff, 0x00020000);
+      p[i] = __builtin_bit_cast(f4, __builtin_amdgcn_raw_buffer_load_b128(rsrc, wi[i] != 0.f ? at : NO_ROW, 0, 0));
     }
-  if (d < D) *reinterpret_cast<typename Ty<T>::Quad*>(out + row * D + d) = __builtin_convertvector(acc, typename Ty<T>::Quad);
-  if (WEIGHTED && d == 0) lse[row] = sum == 0.f ? INF : m + __log2f(sum);
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[e] = fmaf(wi[i], p[i][e], acc[e]);
+  }
+  if (live && d < D) *reinterpret_cast<typename Ty<T>::Quad*>(out + row * D + d) = __builtin_convertvector(acc, typename Ty<T>::Quad);
 }
 
 // -------------------------------------------------------------------------------------------
@@ -519,7 +550,7 @@ __device__ __forceinline__ float pow2_of(uint32_t bits) {   // 2^e of |x|, 1 for
 template <class T, int DP, bool BIAS, int NW>
 __device__ __forceinline__ void dq_body(const Args& a, int wg, int part_no) {
   using L = Tile<T, DP>;
-  constexpr int NT = NW * 64, BN = key_tile<T, DP>(), NB = BN / 32, TILE = BN * L::RB;
+  constexpr int NT = NW * 64, BN = key_tile<T, DP, NW>(), NB = BN / 32, TILE = BN * L::RB;
   constexpr bool HALF = __is_same(T, _Float16);
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int nsplit = a.split_q;
@@ -616,7 +647,7 @@ __device__ __forceinline__ void dq_body(const Args& a, int wg, int part_no) {
         const float c = BIAS ? 1.f : a.c;
         const int rel0 = base - qabs;
         const int lo = base - qfirst - 31, hi = base - qfirst + 31;   // the tile's relative positions
-        if (BIAS) add_bias<1>(s, a.c, lut, rel0, lo, hi, h, R, -lse);
+        if (BIAS) add_bias<1, true>(s, a.c, lut, rel0, lo, hi, h, R, -lse);
 #pragma unroll
         for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c, BIAS ? 0.f : -lse)) * (FROM ? g[r] : g[r] - delta);
         if (base + 32 > wmin) {
@@ -635,7 +666,7 @@ __device__ __forceinline__ void dq_body(const Args& a, int wg, int part_no) {
             // Row i's keys are written i places further left, so that a column holds one distance: lane d
             // sums column d over the 32 rows and adds it to this wave's sums.  (A wave's LDS operations
             // keep their order; places that no key reaches stay zero.  Adding each score atomically took
-            // 280 cycles for 32 of them: 145 us instead of XXX, fp16 training with 12 heads of 64.)
+            // 280 cycles for 32 of them: dQ 145 us instead of 81, fp16 training with 12 heads of 64.)
             float* p = skew + 63 * (lane & 31) + 4 * h + 31;
 #pragma unroll
             for (int r = 0; r < 16; ++r) p[acc_row(r, 0)] = s[r];
@@ -834,7 +865,7 @@ __device__ __forceinline__ void dkv_body(const Args& a, int wg, int part_no) {
       for (int n = 0; n < NB; ++n) {
         if (BIAS) {
           const int lo = key0 + w * 32 - off - rb - 32 * n - 31;
-          add_bias<-1>(s[n], a.c, lut, key - off - rb - 32 * n, lo, lo + 62, h, R);
+          add_bias<-1, false>(s[n], a.c, lut, key - off - rb - 32 * n, lo, lo + 62, h, R);
         }
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
@@ -899,7 +930,9 @@ __device__ __forceinline__ void dkv_body(const Args& a, int wg, int part_no) {
 
 // -------------------------------------------------------------------------------------------
 // backward: both in one launch.  They need nothing of each other but rowsum(dO O) and max |dO|, which
-// delta_kernel takes first, and share the chip to the end instead of each leaving it half empty: XXX
+// delta_kernel takes first, and share the chip to the end instead of each leaving it half empty (training with 12 heads of 64, up to
+// 2047 tokens: dQ 81 and dK / dV 70 us one after the other, 102 together; 10 k tokens, 16 heads of 128 over 4:
+// 818 and 765 us, 0.68 TFLOP counted as seven products: 0.89 PFLOP/s)
 // -------------------------------------------------------------------------------------------
 template <class T, int DP, bool BIAS, int NW>
 __global__ __launch_bounds__(NW * 64, (occ_bwd<T, DP, BIAS, NW>())) void bwd_kernel(Args a) {
@@ -974,7 +1007,7 @@ template <class T, class K> int launch(K kernel, dim3 grid, int threads, size_t 
 
 template <class T, int DP, bool BIAS> int fwd_dp(const Plan& p, hipStream_t s) {
   const Args& a = p.a;
-  const size_t lds = 4 * key_tile<T, DP>() * Tile<T, DP>::RB + (BIAS ? span_of(a.p.max_distance) * 4 : 0);
+  const size_t lds = 4 * (p.nwq == 2 ? key_tile<T, DP, 2>() : key_tile<T, DP, 4>()) * Tile<T, DP>::RB + (BIAS ? span_of(a.p.max_distance) * 4 : 0);
   const int rc = p.nwq == 2 ? launch<T>(fwd_kernel<T, DP, BIAS, 2>, dim3(a.wgs_q, a.split_q), 128, lds, a, s)
                             : launch<T>(fwd_kernel<T, DP, BIAS, 4>, dim3(a.wgs_q, a.split_q), 256, lds, a, s);
   if (rc || a.split_q == 1) return rc;
@@ -990,8 +1023,8 @@ __global__ __launch_bounds__(256) void max_kernel(const float* wgmax, int64_t n,
 
 template <class T, int DP, bool BIAS> int bwd_dp(const Plan& p, hipStream_t s) {
   const Args& a = p.a;
-  constexpr int BN = key_tile<T, DP>(), BQ = row_tile<T, DP>(), RB = Tile<T, DP>::RB;
-  const int R = a.p.max_distance, NH = 2 * R + 1, nw = p.nwq;
+  constexpr int BQ = row_tile<T, DP>(), RB = Tile<T, DP>::RB;
+  const int R = a.p.max_distance, NH = 2 * R + 1, nw = p.nwq, BN = nw == 2 ? key_tile<T, DP, 2>() : key_tile<T, DP, 4>();
   const int64_t blocks = (a.p.total_q + 63) / 64;
   if (blocks > 0) {
     hipLaunchKernelGGL((delta_kernel<T>), dim3((unsigned)blocks, a.p.Hq), dim3(256), 0, s, a);

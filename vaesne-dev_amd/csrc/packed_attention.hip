@@ -44,21 +44,21 @@ __global__ __launch_bounds__(1024) void hist_sum_kernel(const float* hist, int n
 
 namespace {
 
-constexpr int SLOTS = 512;            // workgroups the chip runs at once: two of 64 KB LDS per CU
+constexpr int CUS = 256;
 constexpr int MAX_SPLIT = 64;
 constexpr int64_t MAX_PART = 256 << 20;
 constexpr int64_t MAX_STRIDE = 1 << 21;  // elements: a tile of 128 rows spans less than 2^31 bytes
 constexpr int64_t MAX_ROWS = 1 << 25; // rows of one sequence: 32-bit row arithmetic with room
 
 // Parts to cut the streamed axis into, in units of a tile (about 1.2 us).  Each of `wgs` workgroups walks
-// up to `longest` tiles, `mean` on average; SLOTS of them run at once, longest first, beside `beside`
+// up to `longest` tiles, `mean` on average; `slots` of them run at once, longest first, beside `beside`
 // units of other work.  Parts have the same length for all (a shorter walk has fewer of them), cost about
 // six tiles more each, and are written and read back once (4.5 TB/s) by a joining launch.  The end of the launch is estimated as
-//   max(all tiles and parts / SLOTS + beside + half of the longest part, the longest part) + joining
+//   max(all tiles and parts / slots + beside + half of the longest part, the longest part) + joining
 // and the fewest parts taken that come within a twentieth of the best.  (fp16 training, 6 sequences of up
 // to 2047, 12 heads: one part 48 us forward, two 58 + 17 us; one token over 32 caches of up to 16384
 // keys: one part 0.35 ms, as chosen 0.13.)
-int splits(int64_t wgs, int64_t longest, double mean, int64_t part_bytes, double beside) {
+int splits(int64_t wgs, int64_t longest, double mean, int64_t part_bytes, int slots, double beside) {
   const double over = 6;
   const int64_t most = std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(MAX_SPLIT, longest / 4),
                                                               MAX_PART / std::max<int64_t>(part_bytes, 1)));
@@ -66,7 +66,7 @@ int splits(int64_t wgs, int64_t longest, double mean, int64_t part_bytes, double
     const double own = (double)((longest + n - 1) / n) + over;
     const double join = n > 1 ? 4 + (double)n * part_bytes / 2.7e6 : 0;
     const double parts = std::max(1.0, n * mean / std::max<double>(longest, 1));
-    return std::max(wgs * (mean + parts * over) / SLOTS + beside + 0.5 * own, own) + join;
+    return std::max(wgs * (mean + parts * over) / slots + beside + 0.5 * own, own) + join;
   };
   double least = end(1);
   for (int64_t n = 2; n <= most; ++n) least = std::min(least, end(n));
@@ -122,16 +122,17 @@ int make_plan(const vaesne_packed_attn* a, int backward, Plan* p) {
   p->nwq = backward ? p->nwk : waves_for(rows);
   r.pk_log = log_heads_per_row_tile(a, p->dp, p->nwk);
   r.nsubk = r.group >> r.pk_log;
-  const int bn = a->type == 0 ? 32 : 64;
+  const int bn = a->type == 0 || (p->dp == 128 && p->nwq == 2) ? 32 : 64;   // key_tile()
   const int64_t qrows = a->total_q * a->Hq, krows = a->total_k * a->Hkv;
   const double n = std::max(a->nseq, 1);
   r.wgs_q = a->n_q_tiles * a->Hkv * r.nsub;
   r.wgs_k = backward ? a->n_k_tiles * a->Hkv : 0;
-  const int bp = (a->type != 0 && p->dp == 128 ? 32 : bn) >> r.pk_log;   // row_tile()
+  const int bp = (a->type == 0 || p->dp == 128 ? 32 : 64) >> r.pk_log;     // row_tile()
   const double mean_q = a->total_k / n / bn, mean_k = (double)r.nsubk * a->total_q / n / bp;
+  const int slots = CUS * (p->nwq == 2 ? 4 : 2);                 // workgroups that run at once
   const int64_t long_q = (a->max_k + bn - 1) / bn, long_k = (int64_t)r.nsubk * ((a->max_q + bp - 1) / bp);
-  r.split_q = splits(r.wgs_q, long_q, mean_q, qrows * (a->D + 1) * 4, r.wgs_k * mean_k / SLOTS);
-  r.split_k = splits(r.wgs_k, long_k, mean_k, 2 * krows * a->D * 4, r.wgs_q * mean_q / SLOTS);
+  r.split_q = splits(r.wgs_q, long_q, mean_q, qrows * (a->D + 1) * 4, slots, r.wgs_k * mean_k / slots);
+  r.split_k = splits(r.wgs_k, long_k, mean_k, 2 * krows * a->D * 4, slots, r.wgs_q * mean_q / slots);
   r.per_q = (int)((long_q + r.split_q - 1) / r.split_q);
   r.per_k = (int)((long_k + r.split_k - 1) / r.split_k);
   return 0;
