@@ -640,7 +640,8 @@ int vaesne_gated_norm_bwd(const vaesne_gated_norm* a, void* stream);
  * largest |x|, 1), step = 2^(exps - 133), codes = round-half-even(x / step) clamped to +-127 (the
  * error is at most step / 2, a whole step where 127 clips); exps 255 marks a block with a NaN or an
  * infinity, which reads back as NaN.  codes: int8 [n], exps: uint8 [ceil(n / 32)].
- * gelu8: y = GELU(x) (erf form) beside the codes; its backward reads only them:
+ * gelu8: y = GELU(x) (erf form) beside the codes (codes and exps both null: y alone); its backward reads
+ * only them:
  *   dx = dy GELU'(kept x), and y_again (nullable) = GELU(kept x). */
 int vaesne_pack8(int type, const void* x, int64_t n, int8_t* codes, uint8_t* exps, void* stream);
 int vaesne_unpack8(int type, const int8_t* codes, const uint8_t* exps, int64_t n, void* x, void* stream);

@@ -629,6 +629,17 @@ def test_gelu8(t, shape):
     assert ((d.double() - want).abs() <= u * want.abs() + (1e-7 + 16 * F) * dy.double().abs() * (1 + kept.abs()) + smallest(t)).all()
 
 
+@pytest.mark.parametrize("t", TYPES, ids=str)
+def test_act8_without_gradients_is_the_same(t):
+    g = gen(34)
+    x, W, b = normal(g, 9, 50, dtype=t), normal(g, 20, 50, dtype=t), normal(g, 20, dtype=t)
+    leaf = x.detach().requires_grad_()
+    assert torch.equal(P().gelu8(x), P().gelu8(leaf))
+    for act in (None, "gelu"):
+        assert torch.equal(P().linear8(x, W, b, act=act), P().linear8(leaf, W, b, act=act))
+    assert torch.equal(P().gelu8(x.t()), P().gelu8(x).t())
+
+
 def test_gelu8_far_out():
     x = torch.tensor([float("-inf"), -30.0, -6.0, 0.0, 6.0, 30.0, float("inf"), float("nan")], device="cuda")
     for t in TYPES:

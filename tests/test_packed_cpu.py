@@ -112,7 +112,7 @@ def attn_args(backward=0, **kw):
     dict(type=3), dict(type=-1), dict(Hq=0), dict(Hkv=3), dict(Hkv=0), dict(D=0), dict(D=12), dict(D=136),
     dict(scale=0.0), dict(scale=-1.0), dict(scale=math.nan), dict(q_tile=31), dict(k_tile=64), dict(max_q=1 << 26),
     dict(max_k=1 << 26), dict(total_q=-1), dict(q=None), dict(k=None), dict(o=None), dict(lse=None),
-    dict(q_tiles=None), dict(n_q_tiles=0), dict(q=72), dict(k=66), dict(q_ts=516), dict(v_hs=4), dict(k_ts=1 << 23),
+    dict(q_tiles=None), dict(n_q_tiles=0), dict(n_q_tiles=-1), dict(n_q_tiles=1 << 22), dict(n_k_tiles=1 << 24), dict(q=72), dict(k=66), dict(q_ts=516), dict(v_hs=4), dict(k_ts=1 << 23),
     dict(q_hs=-64), dict(table=64, max_distance=0, num_buckets=4), dict(table=64, max_distance=513, num_buckets=4),
     dict(table=64, max_distance=8, num_buckets=0), dict(table=64, max_distance=8, num_buckets=4, lut=None)])
 def test_attention_entry_refuses(change):
@@ -179,6 +179,7 @@ def test_act8_entries_refuse():
         assert lib.vaesne_gelu8_fwd(t, x, n, 64, codes, exps, None) == BAD
         assert lib.vaesne_gelu8_bwd(t, codes, exps, 64, n, x, None, None) == BAD
     assert lib.vaesne_gelu8_fwd(0, 64, 32, None, 64, 64, None) == BAD
+    assert lib.vaesne_gelu8_fwd(0, 64, 32, 64, None, 64, None) == BAD
     assert lib.vaesne_gelu8_bwd(0, 64, 64, None, 32, 64, None, None) == BAD
     for fn, args in (("pack8", (0, None, 0, None, None)), ("unpack8", (0, None, None, 0, None)),
                      ("gelu8_fwd", (0, None, 0, None, None, None)), ("gelu8_bwd", (0, None, None, None, 0, None, None))):

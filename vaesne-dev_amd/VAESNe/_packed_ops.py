@@ -275,8 +275,10 @@ class RelativeBuckets:
             if torch.cuda.is_current_stream_capturing():
                 raise RuntimeError("RelativeBuckets: the bucket table is not on the device yet and cannot be copied "
                                    "inside a graph capture; run the same call once before capturing")
-            got = self._dev[device] = self.lut.to(device)
-        return got
+            got = self._dev[device] = (self.lut.to(device), torch._C._cuda_getCurrentRawStream(device.index))
+        if torch._C._cuda_getCurrentRawStream(device.index) != got[1]:
+            got[0].record_stream(torch.cuda.current_stream(device))
+        return got[0]
 
     def __getstate__(self):
         return {**self.__dict__, "_dev": {}}
@@ -582,7 +584,17 @@ class Gelu8Fn(torch.autograd.Function):
 def gelu8(x):
     """GELU (erf form) that keeps its input in 8 bits for the backward pass (PackedLayers.gelu8)."""
     _type_of("gelu8", x)
-    return Gelu8Fn.apply(x)
+    if torch.is_grad_enabled() and x.requires_grad:
+        return Gelu8Fn.apply(x)
+    return _gelu(x)
+
+
+def _gelu(x):
+    """GELU alone: nothing is kept."""
+    x = x.contiguous()
+    y = torch.empty_like(x)
+    _lib_call("gelu8_fwd", x.device, TYPES[x.dtype], x.data_ptr(), x.numel(), y.data_ptr(), None, None)
+    return y
 
 
 class Linear8Fn(torch.autograd.Function):
@@ -629,4 +641,6 @@ def linear8(x, weight, bias=None, act=None):
         raise ValueError("linear8: act is None or 'gelu'")
     if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1] or (bias is not None and tuple(bias.shape) != (weight.shape[0],)):
         raise ValueError("linear8: x [.., in], weight [out, in], bias [out]")
-    return Linear8Fn.apply(x, weight, bias, act == "gelu")
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
+        return Linear8Fn.apply(x, weight, bias, act == "gelu")
+    return torch.nn.functional.linear(_gelu(x) if act else x, weight, bias)

@@ -135,7 +135,7 @@ __global__ __launch_bounds__(NT) void keep_kernel(const T* __restrict__ x, int64
                                                   int8_t* __restrict__ codes, uint8_t* __restrict__ exps) {
   const int64_t i = ((int64_t)blockIdx.x * NT + threadIdx.x) * 8;
   f8 v = load8<T, VEC>(x, i, n);
-  encode(v, i, n, codes, exps);
+  if (!GELU || codes) encode(v, i, n, codes, exps);
   if (GELU) {
 #pragma unroll
     for (int k = 0; k < 8; ++k) v[k] = gelu8<T>(v[k]);
@@ -191,7 +191,7 @@ bool bad(int type, int64_t n, const void* codes) {
 }
 
 template <bool GELU> int keep_any(int type, const void* x, int64_t n, void* y, int8_t* codes, uint8_t* exps, void* stream) {
-  if (bad(type, n, codes) || (n > 0 && (!x || !codes || !exps || (GELU && !y)))) return (int)hipErrorInvalidValue;
+  if (bad(type, n, codes) || (n > 0 && (!x || (GELU ? !codes != !exps || !y : !codes || !exps)))) return (int)hipErrorInvalidValue;
   if (n == 0) return 0;
   hipStream_t s = (hipStream_t)stream;
   return type == 0 ? keep<float, GELU>(x, n, y, codes, exps, s)

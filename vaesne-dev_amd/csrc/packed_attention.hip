@@ -125,6 +125,9 @@ int make_plan(const vaesne_packed_attn* a, int backward, Plan* p) {
   const int bn = a->type == 0 || (p->dp == 128 && p->nwq == 2) ? 32 : 64;   // key_tile()
   const int64_t qrows = a->total_q * a->Hq, krows = a->total_k * a->Hkv;
   const double n = std::max(a->nseq, 1);
+  // workgroups of all parts together: below 2^31
+  if (a->n_q_tiles < 0 || a->n_k_tiles < 0 || (int64_t)a->n_q_tiles * a->Hq >= (1 << 24) || (int64_t)a->n_k_tiles * a->Hkv >= (1 << 24))
+    return (int)hipErrorInvalidValue;
   r.wgs_q = a->n_q_tiles * a->Hkv * r.nsub;
   r.wgs_k = backward ? a->n_k_tiles * a->Hkv : 0;
   const int bp = (a->type == 0 || p->dp == 128 ? 32 : 64) >> r.pk_log;     // row_tile()
@@ -174,7 +177,7 @@ int check(const Plan& p, int64_t bytes, int backward) {
   const int size = a.type == 0 ? 4 : 2;
   const int bad = (int)hipErrorInvalidValue;
   if (a.q_tile != p.nwq * 32 / p.a.pg || (backward && a.k_tile != p.nwk * 32)) return bad;
-  if (a.n_q_tiles < 0 || a.n_k_tiles < 0 || (a.total_q > 0 && (a.n_q_tiles == 0 || !a.q_tiles || !a.q || !a.o || !a.lse)) ||
+  if ((a.total_q > 0 && (a.n_q_tiles == 0 || !a.q_tiles || !a.q || !a.o || !a.lse)) ||
       (a.total_k > 0 && (!a.k || !a.v)))
     return bad;
   if (!aligned(a.q, a.q_ts, a.q_hs, size) || !aligned(a.k, a.k_ts, a.k_hs, size) || !aligned(a.v, a.v_ts, a.v_hs, size) ||
@@ -182,7 +185,6 @@ int check(const Plan& p, int64_t bytes, int backward) {
     return bad;
   if (a.table && !a.lut) return bad;
   if (bytes > 0 && (!a.workspace || (reinterpret_cast<uintptr_t>(a.workspace) & 15))) return bad;
-  if ((int64_t)a.n_q_tiles * a.Hq >= (1ll << 31) || (int64_t)a.n_k_tiles * a.Hkv >= (1ll << 31)) return bad;
   if (backward) {
     if (a.total_q > 0 && (!a.dout || !a.dq)) return bad;
     if (a.total_k > 0 && (!a.dk || !a.dv || a.n_k_tiles == 0 || !a.k_tiles)) return bad;
