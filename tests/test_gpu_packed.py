@@ -867,3 +867,103 @@ def test_two_calls_at_once_keep_apart():
                 got[i].append(run_attention(*sets[i], seqs)["o"])
     torch.cuda.synchronize()
     assert all(torch.equal(want[i], o) for i in range(2) for o in got[i])
+
+
+# ------------------------------------------------------------------------------------------------
+# what surrounds the calls: copies, hooks, streams, hand-made arguments
+# ------------------------------------------------------------------------------------------------
+def test_copied_and_pickled_sequences_work_by_themselves():
+    import copy
+    import pickle
+    L, g = P(), gen(70)
+    n = [5, 70, 0, 31]
+    q, k, v, do = (normal(g, sum(n), 4, 32, dtype=torch.bfloat16) for _ in range(4))
+    seqs = L.PackedSequences(n)
+    want = run_attention(q, k, v, seqs, do, causal=True)
+    twins = [copy.deepcopy(seqs), pickle.loads(pickle.dumps(seqs))]
+    del seqs
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    for twin in twins:
+        got = run_attention(q, k, v, twin, do, causal=True)
+        assert all(torch.equal(want[name], got[name]) for name in want)
+
+
+def test_saved_tensors_that_come_back_with_other_strides():
+    """Hooks that keep saved tensors elsewhere return them contiguous."""
+    L, g = P(), gen(71)
+    wide = normal(g, 50, 3, 64)
+    x, f, gate = (wide[:, i].detach().requires_grad_() for i in range(3))
+    w1, w2 = (normal(g, 64, mean=1.0, scale=0.1).requires_grad_() for _ in range(2))
+    dy, dn = normal(g, 50, 64), normal(g, 50, 64)
+    n = [20, 30]
+    qkv = normal(g, 50, 12, 16)
+    q, k, v = (qkv[:, 4 * i:4 * i + 4].detach().requires_grad_() for i in range(3))
+    do = normal(g, 50, 4, 16)
+    h, W = normal(g, 50, 64).requires_grad_(), normal(g, 33, 64).requires_grad_()
+    seqs = L.PackedSequences(n)
+
+    def grads():
+        y, m = L.gated_norm(x, f, w1, w2, gate=gate)
+        a = L.packed_attention(q, k, v, seqs)
+        z = L.linear8(h, W, act="gelu")
+        u = L.gelu8(h)
+        return torch.autograd.grad([y, m, a, z, u], [x, f, gate, w1, w2, q, k, v, h, W],
+                                   [dy, dn, do, torch.ones_like(z), dy])
+    want = grads()
+    with torch.autograd.graph.save_on_cpu():
+        got = grads()
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
+
+
+def test_tables_made_on_one_stream_and_read_on_another():
+    L, g = P(), gen(72)
+    n = [40, 90]
+    q, k, v = (normal(g, 130, 4, 32) for _ in range(3))
+    want = L.packed_attention(q, k, v, L.PackedSequences(n))
+    seqs = L.PackedSequences(n)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        first = L.packed_attention(q, k, v, seqs)
+    assert all(s == side.cuda_stream for call in seqs._calls.values() for _, s in call[2])
+    second = L.packed_attention(q, k, v, seqs)
+    del seqs
+    with torch.cuda.stream(side):
+        spoiled = torch.full((4096,), -1, dtype=torch.int32, device="cuda")     # (where the tables were, if free)
+    torch.cuda.synchronize()
+    assert torch.equal(first, want) and torch.equal(second, want) and int(spoiled[0]) == -1
+
+
+@pytest.mark.parametrize("change", [dict(codes=lambda p: p.codes[:-1]), dict(exponents=lambda p: p.exponents[:-1]),
+                                    dict(codes=lambda p: p.codes.to(torch.int16)), dict(shape=lambda p: torch.Size([41])),
+                                    dict(codes=lambda p: p.codes.repeat(2)[::2]), dict(dtype=lambda p: torch.float64)])
+def test_unpack8_checks_what_it_is_given(change):
+    L = P()
+    p = L.pack8(torch.randn(40, device="cuda"))
+    for name, new in change.items():
+        setattr(p, name, new(p))
+    with pytest.raises(ValueError, match="unpack8"):
+        L.unpack8(p)
+
+
+def test_buckets_must_be_relative_buckets():
+    L = P()
+    seqs = L.PackedSequences([8])
+    q = torch.randn(8, 2, 16, device="cuda")
+    with pytest.raises(TypeError, match="RelativeBuckets"):
+        L.packed_attention(q, q, q, seqs, bias=torch.zeros(8, 2, device="cuda"), buckets=[0] * 8)
+
+
+def test_norm_of_more_rows_than_an_axis_of_a_grid():
+    """A wave a row: 2^26 rows are 2^32 threads.  Rows are independent: the last ones alone give the same."""
+    L, g = P(), gen(73)
+    rows = (1 << 26) + 5
+    x = torch.empty(rows, 2, dtype=torch.float16, device="cuda")
+    x.copy_(torch.arange(rows, device="cuda")[:, None] % 61 - 30)
+    f, w = normal(g, rows, 2, dtype=torch.float16), normal(g, 2, dtype=torch.float16)
+    with torch.no_grad():
+        y, n = L.gated_norm(x, f, w, w)
+        for part in (slice(0, 4099), slice(rows - 4099, rows)):
+            py, pn = L.gated_norm(x[part], f[part], w, w)
+            assert torch.equal(y[part], py) and torch.equal(n[part], pn)

@@ -1,5 +1,6 @@
 """Host side of the packed-sequence operators: bucket tables, tile tables, refusals.  Nothing here
 launches a kernel: every bad argument is turned down before one could run."""
+import copy
 import ctypes as C
 import math
 
@@ -184,3 +185,37 @@ def test_act8_entries_refuse():
     for fn, args in (("pack8", (0, None, 0, None, None)), ("unpack8", (0, None, None, 0, None)),
                      ("gelu8_fwd", (0, None, 0, None, None, None)), ("gelu8_bwd", (0, None, None, None, 0, None, None))):
         assert getattr(lib, "vaesne_" + fn)(*args, None) == 0                      # nothing to do
+
+
+@pytest.mark.parametrize("change", [dict(total_q=1 << 30), dict(total_k=1 << 30),
+                                    dict(n_q_tiles=(1 << 21) - 1, n_k_tiles=(1 << 23) - 1)])
+def test_launches_past_a_grid_are_refused(change):
+    """An axis of a grid has fewer than 2^32 threads."""
+    a = attn_args(1, **change)
+    assert _lib.load().vaesne_packed_attn_bwd(C.addressof(a), None) == BAD
+    lib = _lib.load()
+    n = 1 << 35
+    assert lib.vaesne_pack8(1, 64, n, 64, 64, None) == BAD
+    assert lib.vaesne_unpack8(1, 64, 64, n, 64, None) == BAD
+    assert lib.vaesne_gelu8_fwd(1, 64, n, 64, 64, 64, None) == BAD
+    assert lib.vaesne_gelu8_bwd(1, 64, 64, 64, n, 64, None, None) == BAD
+
+
+@pytest.mark.parametrize("total", [[1 << 30], [1 << 29, 1 << 29]])
+def test_sequences_of_too_many_tokens_are_refused(total):
+    with pytest.raises(ValueError, match="2\\^30"):
+        P.PackedSequences(total, device="cpu")
+
+
+def test_unpack8_refuses_codes_on_the_host():
+    kept = P.Packed8(torch.zeros(40, dtype=torch.int8), torch.zeros(2, dtype=torch.uint8), torch.Size([40]), torch.float32)
+    with pytest.raises(RuntimeError, match="ROCm"):
+        P.unpack8(kept)
+
+
+def test_a_copy_of_sequences_makes_its_own_tables():
+    seqs = object.__new__(P.PackedSequences)
+    seqs.__dict__.update(lengths=[3], _tables={"a": 1}, _calls={"b": 2}, _index=None)
+    twin = copy.deepcopy(seqs)
+    assert twin.lengths == [3] and twin._tables == {} and twin._calls == {}
+    assert seqs._tables == {"a": 1} and seqs._calls == {"b": 2}

@@ -98,8 +98,8 @@ def _lengths(lengths, name):
     out = [int(n) for n in lengths]
     if any(n < 0 or n != m for n, m in zip(out, lengths)):
         raise ValueError(f"PackedSequences: {name} are whole numbers from 0 up")
-    if sum(out) >= 1 << 31:
-        raise ValueError(f"PackedSequences: {name} add up to 2^31 or more tokens")
+    if sum(out) >= 1 << 30:
+        raise ValueError(f"PackedSequences: {name} add up to 2^30 or more tokens")
     return out
 
 
@@ -150,7 +150,10 @@ class PackedSequences:
         self._tables = {}
         self._calls = {}
         self._index = None
-        self._stream = torch._C._cuda_getCurrentRawStream(self.device.index)
+
+    def __getstate__(self):
+        # a copy makes its own tables: the kept calls hold the addresses of this one's
+        return {**self.__dict__, "_tables": {}, "_calls": {}}
 
     @classmethod
     def from_mask(cls, mask):
@@ -161,24 +164,28 @@ class PackedSequences:
         if mask.dim() != 2:
             raise ValueError("PackedSequences.from_mask: mask is [B, L]")
         keep = mask == 0 if mask.dtype != torch.bool else ~mask
-        out = cls(keep.sum(1).tolist(), device=mask.device)
-        out._index = (torch.nonzero(keep.reshape(-1)).reshape(-1), tuple(mask.shape))
+        at = torch.nonzero(keep.reshape(-1)).reshape(-1)
+        out = cls(keep.sum(1).tolist(), device=mask.device)  # (waits for `at` too: any stream may read it)
+        out._index = (at, tuple(mask.shape))
         return out
+
+    def _indexes(self, name):
+        """from_mask's places and shape; the places are noted on the stream that will read them."""
+        if self._index is None:
+            raise RuntimeError(f"PackedSequences.{name}: only for sequences made by from_mask")
+        self._index[0].record_stream(torch.cuda.current_stream(self.device))
+        return self._index
 
     def pack(self, x):
         """Padded [B, L, ...] -> packed [total, ...] (from_mask's sequences)."""
-        if self._index is None:
-            raise RuntimeError("PackedSequences.pack: only for sequences made by from_mask")
-        at, shape = self._index
+        at, shape = self._indexes("pack")
         if tuple(x.shape[:2]) != shape:
             raise ValueError(f"PackedSequences.pack: x is {tuple(x.shape)}, the mask was {shape}")
         return x.reshape(shape[0] * shape[1], *x.shape[2:]).index_select(0, at)
 
     def unpack(self, x):
         """Packed [total, ...] -> padded [B, L, ...], zeros in the masked places."""
-        if self._index is None:
-            raise RuntimeError("PackedSequences.unpack: only for sequences made by from_mask")
-        at, shape = self._index
+        at, shape = self._indexes("unpack")
         if x.shape[0] != self.total:
             raise ValueError(f"PackedSequences.unpack: x has {x.shape[0]} rows, the sequences {self.total}")
         out = x.new_zeros((shape[0] * shape[1], *x.shape[1:])).index_copy(0, at, x)
@@ -191,12 +198,13 @@ class PackedSequences:
         return torch.from_numpy(array).to(self.device)       # (waits for the copy: any stream may read it)
 
     def _table(self, side, tile, causal):
-        """tile_table's rows on the device, and how many."""
+        """tile_table's rows on the device, how many, and the stream whose memory they are in."""
         key = (side, tile, bool(causal))
         got = self._tables.get(key)
         if got is None:
             table = tile_table(self._q, self._k, side, tile, causal)
-            got = self._tables[key] = (self._upload(table.reshape(-1)) if len(table) else None, len(table))
+            got = self._tables[key] = (self._upload(table.reshape(-1)) if len(table) else None, len(table),
+                                       torch._C._cuda_getCurrentRawStream(self.device.index))
         return got
 
     def _call(self, type_, Hq, Hkv, D, causal, buckets, backward):
@@ -221,15 +229,15 @@ class PackedSequences:
             if ws < 0:
                 raise RuntimeError("packed_attention: sizes out of range")
             a.table = a.dtable = None
-            got = self._calls[key] = (bytes(a), ws, [t for t, _ in tables if t is not None])
+            got = self._calls[key] = (bytes(a), ws, [(t, s) for t, _, s in tables if t is not None])
         return got
 
     def _args(self, call):
         """A fresh argument struct of `call`; the tables are noted on the stream that will read them."""
-        if torch._C._cuda_getCurrentRawStream(self.device.index) != self._stream:
-            cur = torch.cuda.current_stream(self.device)
-            for t in call[2]:
-                t.record_stream(cur)
+        raw = torch._C._cuda_getCurrentRawStream(self.device.index)
+        for t, stream in call[2]:
+            if stream != raw:
+                t.record_stream(torch.cuda.current_stream(self.device))
         return _AttnArgs.from_buffer_copy(call[0])
 
 
@@ -372,6 +380,8 @@ def packed_attention(q, k, v, seqs, causal=False, scale=None, bias=None, buckets
         raise ValueError("packed_attention: bias and buckets go together")
     lut = None
     if bias is not None:
+        if not isinstance(buckets, RelativeBuckets):
+            raise TypeError("packed_attention: buckets is a RelativeBuckets")
         if tuple(bias.shape) != (buckets.num_buckets, Hq):
             raise ValueError(f"packed_attention: bias is [buckets, heads] = {(buckets.num_buckets, Hq)}, not "
                              f"{tuple(bias.shape)}")
@@ -427,7 +437,7 @@ class GatedNormFn(torch.autograd.Function):
         a, held, rows = _norm_args(x, branch, pre_w, post_w, pre_b, post_b, gate, scale, kind, eps, type_)
         y, n, stats = _norm_fwd(a, x, branch, rows, True)
         ctx.meta = (scale, kind, eps, type_, rows, x.shape, None if gate is None else gate.shape)
-        ctx.lds = (a.ldx, a.ldbranch, a.ldgate, a.gate_kind)
+        ctx.gate_kind = a.gate_kind
         ctx.save_for_backward(*held, stats)
         ctx.set_materialize_grads(False)
         return n if branch is None else (y, n)
@@ -437,7 +447,10 @@ class GatedNormFn(torch.autograd.Function):
     def backward(ctx, *grads):
         xr, br, gr, pre_w, pre_b, post_w, post_b, stats = ctx.saved_tensors
         scale, kind, eps, type_, rows, shape, gshape = ctx.meta
-        ldx, ldb, ldg, gk = ctx.lds
+        gk = ctx.gate_kind
+        # (saved tensors may come back with other strides: hooks that keep them elsewhere)
+        (xr, _, ldx), (br, _, ldb) = _rows(xr), (None, 0, 0) if br is None else _rows(br)
+        gr, _, ldg = (gr, 0, 0) if gk != 2 else _rows(gr)
         dy, dn = (None, grads[0]) if br is None else grads
         if dy is None and dn is None:
             return (None,) * 11
@@ -542,6 +555,13 @@ def unpack8(packed):
     """The values that a Packed8 stands for, in its own shape and type."""
     if not isinstance(packed, Packed8):
         raise TypeError("unpack8: takes what pack8 returns")
+    codes, exps, n = packed.codes, packed.exponents, math.prod(packed.shape)
+    _lib.require_device(codes, exps)
+    if codes.device != exps.device or packed.dtype not in TYPES:
+        raise ValueError("unpack8: codes and exponents on one device, of a float32, bfloat16 or float16 tensor")
+    if (codes.dtype != torch.int8 or exps.dtype != torch.uint8 or codes.numel() != n or exps.numel() != (n + 31) // 32 or
+            not codes.is_contiguous() or not exps.is_contiguous()):
+        raise ValueError(f"unpack8: {n} values are {n} int8 codes and {(n + 31) // 32} uint8 exponents, each contiguous")
     return _unpack(packed.codes, packed.exponents, packed.shape, packed.dtype)
 
 

@@ -185,9 +185,9 @@ int back(const int8_t* codes, const uint8_t* exps, const void* dy, int64_t n, vo
   VAESNE_CHECK_LAUNCH();
   return 0;
 }
-// codes are stored 8 at a time; a launch holds 2^31 - 1 workgroups
+// codes are stored 8 at a time; an axis of a grid has fewer than 2^32 threads
 bool bad(int type, int64_t n, const void* codes) {
-  return type < 0 || type > 2 || n < 0 || (reinterpret_cast<uintptr_t>(codes) & 7) || n / (NT * 8) >= (1ll << 31) - 1;
+  return type < 0 || type > 2 || n < 0 || (reinterpret_cast<uintptr_t>(codes) & 7) || n / (NT * 8) >= (1ll << 24) - 1;
 }
 
 template <bool GELU> int keep_any(int type, const void* x, int64_t n, void* y, int8_t* codes, uint8_t* exps, void* stream) {

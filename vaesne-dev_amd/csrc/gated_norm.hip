@@ -138,7 +138,7 @@ template <class T, int P, int V, int NV> __global__ __launch_bounds__(NT<P>) voi
   constexpr int RPB = NT<P> / P;
   const vaesne_gated_norm& p = a.p;
   const int tid = threadIdx.x % P, C = p.C;
-  const int64_t r = (int64_t)blockIdx.x * RPB + threadIdx.x / P;
+  const int64_t r = ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * RPB + threadIdx.x / P;
   const bool live = r < p.rows, layer = p.kind == 1;
   if (WHOLE<P> && !live) return;                       // (whole workgroups only)
   Chunk<T, V> x[NV], f[NV];
@@ -436,7 +436,9 @@ int chunk_of(const vaesne_gated_norm& a) {
 template <class T, int P, int V, int NV> int go(const NArgs& a, bool backward, hipStream_t s) {
   const int64_t rpb = NT<P> / P;
   if (!backward) {
-    hipLaunchKernelGGL((fwd_kernel<T, P, V, NV>), dim3((unsigned)((a.p.rows + rpb - 1) / rpb)), dim3(NT<P>), 0, s, a);
+    // (an axis of a grid has fewer than 2^32 threads: workgroups past 2^22 go to the second)
+    const int64_t wgs = (a.p.rows + rpb - 1) / rpb, wide = std::min<int64_t>(wgs, 1 << 22);
+    hipLaunchKernelGGL((fwd_kernel<T, P, V, NV>), dim3((unsigned)wide, (unsigned)((wgs + wide - 1) / wide)), dim3(NT<P>), 0, s, a);
     VAESNE_CHECK_LAUNCH();
     return 0;
   }

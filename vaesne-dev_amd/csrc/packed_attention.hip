@@ -48,6 +48,7 @@ constexpr int CUS = 256;
 constexpr int MAX_SPLIT = 64;
 constexpr int64_t MAX_PART = 256 << 20;
 constexpr int64_t MAX_STRIDE = 1 << 21;  // elements: a tile of 128 rows spans less than 2^31 bytes
+constexpr int64_t MAX_TOKENS = 1 << 30;  // 4 threads of a launch each; an axis of a grid has fewer than 2^32
 constexpr int64_t MAX_ROWS = 1 << 25; // rows of one sequence: 32-bit row arithmetic with room
 
 // Parts to cut the streamed axis into, in units of a tile (about 1.2 us).  Each of `wgs` workgroups walks
@@ -80,7 +81,7 @@ int64_t up16(int64_t n) { return (n + 15) & ~(int64_t)15; }
 bool sizes_ok(const vaesne_packed_attn* a) {
   return a && a->type >= 0 && a->type <= 2 && a->Hq > 0 && a->Hkv > 0 && a->Hq % a->Hkv == 0 && a->D > 0 &&
          a->D <= 128 && a->D % 8 == 0 && a->nseq >= 0 && a->max_q >= 0 && a->max_k >= 0 && a->total_q >= 0 &&
-         a->total_k >= 0 && a->scale > 0.f && a->Hq <= 4096 &&
+         a->total_k >= 0 && a->total_q < MAX_TOKENS && a->total_k < MAX_TOKENS && a->scale > 0.f && a->Hq <= 4096 &&
          (a->table == nullptr || (a->max_distance >= 1 && a->max_distance <= 512 && a->num_buckets >= 1));
 }
 
@@ -125,7 +126,7 @@ int make_plan(const vaesne_packed_attn* a, int backward, Plan* p) {
   const int bn = a->type == 0 || (p->dp == 128 && p->nwq == 2) ? 32 : 64;   // key_tile()
   const int64_t qrows = a->total_q * a->Hq, krows = a->total_k * a->Hkv;
   const double n = std::max(a->nseq, 1);
-  // workgroups of all parts together: below 2^31
+  // a launch's workgroups of at most 256 threads: below 2^32 threads
   if (a->n_q_tiles < 0 || a->n_k_tiles < 0 || (int64_t)a->n_q_tiles * a->Hq >= (1 << 24) || (int64_t)a->n_k_tiles * a->Hkv >= (1 << 24))
     return (int)hipErrorInvalidValue;
   r.wgs_q = a->n_q_tiles * a->Hkv * r.nsub;
@@ -136,6 +137,8 @@ int make_plan(const vaesne_packed_attn* a, int backward, Plan* p) {
   const int64_t long_q = (a->max_k + bn - 1) / bn, long_k = (int64_t)r.nsubk * ((a->max_q + bp - 1) / bp);
   r.split_q = splits(r.wgs_q, long_q, mean_q, qrows * (a->D + 1) * 4, slots, r.wgs_k * mean_k / slots);
   r.split_k = splits(r.wgs_k, long_k, mean_k, 2 * krows * a->D * 4, slots, r.wgs_q * mean_q / slots);
+  if (backward && ((int64_t)r.wgs_q * r.split_q + (int64_t)r.wgs_k * r.split_k) * p->nwk * 64 >= 1ll << 32)
+    return (int)hipErrorInvalidValue;
   r.per_q = (int)((long_q + r.split_q - 1) / r.split_q);
   r.per_k = (int)((long_k + r.split_k - 1) / r.split_k);
   return 0;
