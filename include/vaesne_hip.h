@@ -15,7 +15,8 @@
  *     asynchronously on `stream` (a hipStream_t; pass torch's current stream);
  *   - tensors are fp32 device pointers with explicit element strides
  *     (ld* = row stride, *_bs = batch stride); masks are uint8 (1 = ignore);
- *     band indices are int64;
+ *     band indices are int64; entry points with a `type` take fp32, bf16 or fp16
+ *     (0, 1, 2);
  *   - no function allocates: workspaces are caller-provided, sized by the
  *     matching *_workspace() query;
  *   - `rng_state` is a device int64[2] {seed, counter}; `call_id` names the
@@ -580,7 +581,7 @@ int vaesne_pack(const float* const* srcs, const int64_t* offs, const int64_t* ns
  *   S = scale q k^T + table[lut[clamp(j - i - (nk - nq), -R, R) + R], head]   (table: nullable)
  *   causal: key j is seen iff j <= i + nk - nq;  o = softmax(S) v, 0 where nothing is seen.
  * Query head h reads key head h / (Hq / Hkv).  type: 0 fp32, 1 bf16, 2 fp16 (every tensor but the
- * fp32 statistics has it).  D: a multiple of 8, at most 128.
+ * fp32 statistics has it).  D: a multiple of 8, at most 128.  total_q, total_k < 2^30.
  * q_tiles / k_tiles [n][8]: one row for every tile of q_tile positions / k_tile keys of a sequence, in any
  * order (longest work first is fastest): {first query token, first key token, queries, keys of the
  * sequence, first position of the tile, 0, 0, 0}; vaesne_packed_attn_tiles gives q_tile and k_tile. */
@@ -636,7 +637,7 @@ int vaesne_gated_norm_fwd(const vaesne_gated_norm* a, void* stream);
 int vaesne_gated_norm_bwd(const vaesne_gated_norm* a, void* stream);
 
 /* ---- activations kept in 8 bits -----------------------------------------------
- * Blocks of 32 consecutive values share a power of two: exps[i] = max(exponent field of the block's
+ * n < 2^35.  Blocks of 32 consecutive values share a power of two: exps[i] = max(exponent field of the block's
  * largest |x|, 1), step = 2^(exps - 133), codes = round-half-even(x / step) clamped to +-127 (the
  * error is at most step / 2, a whole step where 127 clips); exps 255 marks a block with a NaN or an
  * infinity, which reads back as NaN.  codes: int8 [n], exps: uint8 [ceil(n / 32)].
