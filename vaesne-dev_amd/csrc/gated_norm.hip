@@ -9,7 +9,8 @@
 //   db1 = sum e
 // y is computed again from x and f (the same bytes as reading it back, and unrounded).  A workgroup
 // walks rows and keeps its columns' parameter sums in fp32 registers; the workgroups' partial sums
-// are added in a fixed order.  Bound by HBM: forward 4, backward 6 passes over [rows, C].
+// are added in a fixed order.  Bound by HBM: forward 4, backward 6 passes over [rows, C], 5 and 8 with a gate per
+// token (16384 x 4096 bf16, such a gate: 118 and 240 us, 5.7 and 4.5 TB/s; a copy of 1 GiB reaches 5.2).
 #include <algorithm>
 
 #include "common.h"
@@ -380,36 +381,38 @@ template <class T, int P, int V, int NV, bool LAYER> __global__ __launch_bounds_
 }
 
 struct Outs { void* o[5]; };
-// parameter gradients from the workgroups' partial sums: 64 columns, 16 slices of the workgroups in
-// order, then the slices in order
+// parameter gradients from the workgroups' partial sums: 32 columns, 32 slices of the workgroups in
+// order, then the slices in order (25 MB of partial sums at 4096 columns: 7.5 us; 64 columns and 16
+// slices leave CUs without a workgroup: 11.5)
 template <class T> __global__ __launch_bounds__(1024) void param_kernel(const float* partial, int G, int C, Outs outs) {
   T* out = reinterpret_cast<T*>(outs.o[blockIdx.y]);
   if (!out) return;
-  __shared__ float part[16][64];
-  const int c = blockIdx.x * 64 + (threadIdx.x & 63), slice = threadIdx.x >> 6;
+  __shared__ float part[32][32];
+  const int c = blockIdx.x * 32 + (threadIdx.x & 31), slice = threadIdx.x >> 5;
   float x = 0.f;
   if (c < C)
-    for (int g = slice; g < G; g += 16) x += partial[((int64_t)g * 5 + blockIdx.y) * C + c];
-  part[slice][threadIdx.x & 63] = x;
+    for (int g = slice; g < G; g += 32) x += partial[((int64_t)g * 5 + blockIdx.y) * C + c];
+  part[slice][threadIdx.x & 31] = x;
   __syncthreads();
   if (slice == 0 && c < C) {
     x = 0.f;
-    for (int i = 0; i < 16; ++i) x += part[i][threadIdx.x];
+    for (int i = 0; i < 32; ++i) x += part[i][threadIdx.x];
     out[c] = (T)x;
   }
 }
 
 // threads per row: 8 for the models' own widths, a wave, then a workgroup; at most 16 columns each (with 32
-// the backward's sums and the rows ahead spill)
+// the backward's sums and the rows ahead spill).  A row of 256 to 512 chunks: one chunk a thread in the
+// forward (16384 x 4096 bf16: 118 us, two 123), two in the backward (240 us, one 256: eight waves wait on every sum)
 struct Shape { int V, P, NV; };
-Shape shape_of(int C, int V) {
+Shape shape_of(int C, int V, bool backward) {
   const int n = (C + V - 1) / V;
   if (V > 1 && n <= 8) return {V, 8, 1};
   if (V == 1) return n <= 256 ? Shape{1, 64, 4} : n <= 2048 ? Shape{1, 256, 8} : Shape{1, 512, 16};
   if (n <= 64) return {V, 64, 1};
   if (n <= 128) return {V, 64, 2};
   if (n <= 256) return {V, V == 4 ? 64 : 256, V == 4 ? 4 : 1};
-  if (n <= 512) return {V, 256, 2};
+  if (n <= 512) return backward ? Shape{V, 256, 2} : Shape{V, 512, 1};
   return n <= 1024 ? Shape{V, 512, 2} : Shape{V, 512, 4};
 }
 int groups_of(const vaesne_gated_norm& a, int P) {
@@ -433,22 +436,23 @@ int chunk_of(const vaesne_gated_norm& a) {
   return (m & 15) == 0 && l % V == 0 ? V : 1;
 }
 
-template <class T, int P, int V, int NV> int go(const NArgs& a, bool backward, hipStream_t s) {
+template <class T, int P, int V, int NV> int go_fwd(const NArgs& a, hipStream_t s) {
   const int64_t rpb = NT<P> / P;
-  if (!backward) {
-    // (an axis of a grid has fewer than 2^32 threads: workgroups past 2^22 go to the second)
-    const int64_t wgs = (a.p.rows + rpb - 1) / rpb, wide = std::min<int64_t>(wgs, 1 << 22);
-    hipLaunchKernelGGL((fwd_kernel<T, P, V, NV>), dim3((unsigned)wide, (unsigned)((wgs + wide - 1) / wide)), dim3(NT<P>), 0, s, a);
-    VAESNE_CHECK_LAUNCH();
-    return 0;
-  }
+  // (an axis of a grid has fewer than 2^32 threads: workgroups past 2^22 go to the second)
+  const int64_t wgs = (a.p.rows + rpb - 1) / rpb, wide = std::min<int64_t>(wgs, 1 << 22);
+  hipLaunchKernelGGL((fwd_kernel<T, P, V, NV>), dim3((unsigned)wide, (unsigned)((wgs + wide - 1) / wide)), dim3(NT<P>), 0, s, a);
+  VAESNE_CHECK_LAUNCH();
+  return 0;
+}
+
+template <class T, int P, int V, int NV> int go_bwd(const NArgs& a, hipStream_t s) {
   const int G = groups_of(a.p, P);
   if (a.p.kind) hipLaunchKernelGGL((bwd_kernel<T, P, V, NV, true>), dim3(G), dim3(NT<P>), 0, s, a);
   else hipLaunchKernelGGL((bwd_kernel<T, P, V, NV, false>), dim3(G), dim3(NT<P>), 0, s, a);
   VAESNE_CHECK_LAUNCH();
   Outs o = {{a.p.dpre_w, a.p.dpost_w, a.p.gate_kind == 1 ? a.p.dgate : nullptr, a.p.kind ? a.p.dpre_b : nullptr,
              a.p.kind ? a.p.dpost_b : nullptr}};
-  hipLaunchKernelGGL((param_kernel<T>), dim3((a.p.C + 63) / 64, a.p.kind ? 5 : 3), dim3(1024), 0, s, a.partial, G, a.p.C, o);
+  hipLaunchKernelGGL((param_kernel<T>), dim3((a.p.C + 31) / 32, a.p.kind ? 5 : 3), dim3(1024), 0, s, a.partial, G, a.p.C, o);
   VAESNE_CHECK_LAUNCH();
   return 0;
 }
@@ -456,13 +460,17 @@ template <class T, int P, int V, int NV> int go(const NArgs& a, bool backward, h
 template <class T> int run(const vaesne_gated_norm& p, bool backward, hipStream_t s) {
   constexpr int W = 16 / sizeof(T);
   const NArgs a{p, reinterpret_cast<float*>(p.workspace)};
-  const Shape q = shape_of(p.C, chunk_of(p));
-#define VAESNE_GN(PV, VV, NVV) if (q.P == PV && q.V == VV && q.NV == NVV) return go<T, PV, VV, NVV>(a, backward, s);
-  VAESNE_GN(8, W, 1) VAESNE_GN(64, W, 1) VAESNE_GN(64, W, 2) VAESNE_GN(256, W, 2) VAESNE_GN(512, W, 2)
+  const Shape q = shape_of(p.C, chunk_of(p), backward);
+#define VAESNE_GN_FWD(PV, VV, NVV) if (!backward && q.P == PV && q.V == VV && q.NV == NVV) return go_fwd<T, PV, VV, NVV>(a, s);
+#define VAESNE_GN_BWD(PV, VV, NVV) if (backward && q.P == PV && q.V == VV && q.NV == NVV) return go_bwd<T, PV, VV, NVV>(a, s);
+#define VAESNE_GN(PV, VV, NVV) VAESNE_GN_FWD(PV, VV, NVV) VAESNE_GN_BWD(PV, VV, NVV)
+  VAESNE_GN(8, W, 1) VAESNE_GN(64, W, 1) VAESNE_GN(64, W, 2) VAESNE_GN_FWD(512, W, 1) VAESNE_GN_BWD(256, W, 2) VAESNE_GN(512, W, 2)
   if constexpr (W == 4) { VAESNE_GN(64, W, 4) VAESNE_GN(512, W, 4) }
   else { VAESNE_GN(256, W, 1) }
   VAESNE_GN(64, 1, 4) VAESNE_GN(256, 1, 8) VAESNE_GN(512, 1, 16)
 #undef VAESNE_GN
+#undef VAESNE_GN_BWD
+#undef VAESNE_GN_FWD
   return (int)hipErrorInvalidValue;
 }
 
