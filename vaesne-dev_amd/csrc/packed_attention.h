@@ -90,7 +90,7 @@ __device__ __forceinline__ f16v mma(f4 a, f4 b, f16v c) {
 
 // accumulator registers of contraction block t as the other operand's fragment.  16-bit types
 // round to nearest even here: P <= 2^8 and dS enter the matrix cores in the inputs' own type, the
-// sums stay fp32 (a relative 2^-9 (bf16) of each term, independent between terms)
+// sums stay fp32 (a relative 2^-8 (bf16), 2^-11 (fp16) of each term at most, independent between terms)
 template <class T> __device__ __forceinline__ typename Ty<T>::Frag take(const f16v& s, int t) {
   constexpr int N = 16 / sizeof(T);
   float __attribute__((ext_vector_type(N))) v;
@@ -99,8 +99,18 @@ template <class T> __device__ __forceinline__ typename Ty<T>::Frag take(const f1
   return __builtin_convertvector(v, typename Ty<T>::Frag);
 }
 
+// what take() left behind, for a second product
+template <class T> __device__ __forceinline__ typename Ty<T>::Frag rest_of(const f16v& s, int t, const typename Ty<T>::Frag& taken) {
+  constexpr int N = 16 / sizeof(T);
+  float __attribute__((ext_vector_type(N))) v;
+#pragma unroll
+  for (int j = 0; j < N; ++j) v[j] = s[N * t + j] - (float)taken[j];
+  return __builtin_convertvector(v, typename Ty<T>::Frag);
+}
+
 // ---- LDS tiles -----------------------------------------------------------------------------
 template <class T, int DP> struct Tile {
+  using Type = T;
   static constexpr int EPC = 16 / sizeof(T);          // elements per chunk
   static constexpr int CPR = DP / EPC;                // chunks per row
   static constexpr int RB = CPR * 16;                 // bytes per row
@@ -212,14 +222,14 @@ __device__ __forceinline__ void loads_done() { __builtin_amdgcn_s_waitcnt(0x0f70
 template <int N> struct Int { static constexpr int value = N; };
 
 // Orders the LDS reads of the N fragment products before it: AHEAD fragments (PER reads each) are in
-// flight before the first product, then each product is followed by the next fragment's reads.
+// flight before the first product, then each product (MUL of them a fragment) is followed by the next fragment's reads.
 // (Left to itself the compiler reads, waits and multiplies one fragment at a time.)
-template <int N, int PER, int AHEAD> __device__ __forceinline__ void feed() {
+template <int N, int PER, int AHEAD, int MUL = 1> __device__ __forceinline__ void feed() {
   constexpr int A = AHEAD < N ? AHEAD : N;
   __builtin_amdgcn_sched_group_barrier(0x100, A * PER, 0);
 #pragma unroll
   for (int i = 0; i < N; ++i) {
-    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+    __builtin_amdgcn_sched_group_barrier(0x008, MUL, 0);
     if (i + A < N) __builtin_amdgcn_sched_group_barrier(0x100, PER, 0);
   }
 }
@@ -556,6 +566,26 @@ __device__ __forceinline__ float pow2_of(uint32_t bits) {   // 2^e of |x|, 1 for
   return e == 0 || e >= 255 ? 1.f : __uint_as_float(e << 23);
 }
 
+// acc += X^T dS over the rows of contraction block t.  fp16's dS goes in two parts: rounded once it would be off
+// as much as the gradient's own rounding (1.5 roundings in all, so 1.1), and fp16 is chosen for its
+// digits (training, 12 heads of 64: the launch 102 -> 112 us).  bf16 keeps one part.
+template <class L, class Lane> __device__ __forceinline__ void add_ds(f16v (&acc)[L::DT], const char* x, const Lane& at, int row0, int t, const f16v& ds) {
+  using T = typename L::Type;
+  const auto whole = take<T>(ds, t);
+  if constexpr (__is_same(T, _Float16)) {
+    const auto rest = rest_of<T>(ds, t, whole);
+#pragma unroll
+    for (int dt = 0; dt < L::DT; ++dt) {
+      const auto xt = L::col(x, at, row0, t, dt);
+      acc[dt] = mma(xt, whole, acc[dt]);
+      acc[dt] = mma(xt, rest, acc[dt]);
+    }
+  } else {
+#pragma unroll
+    for (int dt = 0; dt < L::DT; ++dt) acc[dt] = mma(L::col(x, at, row0, t, dt), whole, acc[dt]);
+  }
+}
+
 template <class T, int DP, bool BIAS, int NW>
 __device__ __forceinline__ void dq_body(const Args& a, int wg, int part_no) {
   using L = Tile<T, DP>;
@@ -693,11 +723,9 @@ __device__ __forceinline__ void dq_body(const Args& a, int wg, int part_no) {
         }
 #pragma unroll
         for (int b = 0; b < L::TB; ++b) {
-          const auto sf = take<T>(s, b);
-#pragma unroll
-          for (int dt = 0; dt < L::DT; ++dt) o[dt] = mma(L::col(K, at, 32 * n, b, dt), sf, o[dt]);
+          add_ds<L>(o, K, at, 32 * n, b, s);
         }
-        feed<L::TB * L::DT, L::CR, 3>();
+        feed<L::TB * L::DT, L::CR, 3, HALF ? 2 : 1>();
       }
     }
     if (j + 1 < t1) {
@@ -912,11 +940,9 @@ __device__ __forceinline__ void dkv_body(const Args& a, int wg, int part_no) {
         for (int r = 0; r < 16; ++r) s[n][r] *= HALF ? g[n][r] * down : g[n][r];
 #pragma unroll
         for (int t = 0; t < L::TB; ++t) {
-          const auto sf = take<T>(s[n], t);
-#pragma unroll
-          for (int dt = 0; dt < L::DT; ++dt) dk[dt] = mma(L::col(Q, at, 32 * n, t, dt), sf, dk[dt]);
+          add_ds<L>(dk, Q, at, 32 * n, t, s[n]);
         }
-        feed<L::DT * L::TB, L::CR, 3>();
+        feed<L::DT * L::TB, L::CR, 3, HALF ? 2 : 1>();
       }
     }
     if (it + 1 < t1) commit(1 - b);
@@ -940,7 +966,7 @@ __device__ __forceinline__ void dkv_body(const Args& a, int wg, int part_no) {
 // -------------------------------------------------------------------------------------------
 // backward: both in one launch.  They need nothing of each other but rowsum(dO O) and max |dO|, which
 // delta_kernel takes first, and share the chip to the end instead of each leaving it half empty (training with 12 heads of 64, up to
-// 2047 tokens: dQ 81 and dK / dV 70 us one after the other, 102 together; 10 k tokens, 16 heads of 128 over 4:
+// 2047 tokens, dS in one part: dQ 81 and dK / dV 70 us one after the other, 102 together; 10 k tokens, 16 heads of 128 over 4:
 // 818 and 765 us, 0.68 TFLOP counted as seven products: 0.89 PFLOP/s)
 // -------------------------------------------------------------------------------------------
 template <class T, int DP, bool BIAS, int NW>
