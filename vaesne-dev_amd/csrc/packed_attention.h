@@ -568,7 +568,8 @@ __device__ __forceinline__ float pow2_of(uint32_t bits) {   // 2^e of |x|, 1 for
 
 // acc += X^T dS over the rows of contraction block t.  fp16's dS goes in two parts: rounded once it would be off
 // as much as the gradient's own rounding (1.5 roundings in all, so 1.1), and fp16 is chosen for its
-// digits (training, 12 heads of 64: the launch 102 -> 112 us).  bf16 keeps one part.
+// digits (training, 12 heads of 64: the launch 102 -> 112 us).  bf16 keeps one part
+// (10 k tokens, 16 heads of 128 over 4: two would take 910 us instead of 765).
 template <class L, class Lane> __device__ __forceinline__ void add_ds(f16v (&acc)[L::DT], const char* x, const Lane& at, int row0, int t, const f16v& ds) {
   using T = typename L::Type;
   const auto whole = take<T>(ds, t);
