@@ -5,8 +5,8 @@ stream is filed under that stream, and hipStreamEndCapture walks those files
 recursively: two non-origin streams that wait on each other -- directly, or through
 autograd, which replays each op's backward on its forward stream and so reverses
 every cross-stream edge of the forward -- recurse until the host stack overflows
-(tools/capture_patterns.py: 7 of 9 fork / join shapes end in SIGSEGV inside
-hipStreamEndCapture; DESIGN.md "The backward tail and the graph executor").
+(7 of 9 fork / join shapes tried end the process inside hipStreamEndCapture;
+tests/test_stepgraph_cpu.py holds them as edge lists, checked without a GPU).
 
 The product's captures (training_step's step graphs, bench.py's step) fork every
 side stream from the origin and join it back into the origin only.  `guarded()`
