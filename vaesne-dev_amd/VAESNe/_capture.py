@@ -84,3 +84,24 @@ def guarded(origin=None):
         _active.pop()
         if not _active:
             E.record, E.wait = rec, wait
+
+
+_whole_step = 0
+
+
+@contextlib.contextmanager
+def whole_step():
+    """training_step's own capture of a step, whose later batches replay it without running Python."""
+    global _whole_step
+    _whole_step += 1
+    try:
+        yield
+    finally:
+        _whole_step -= 1
+
+
+def refuse_in_step(name):
+    """Raise where `name`, which differs from batch to batch, would be kept by training_step's own capture
+    (the step then runs eagerly).  A capture that the caller makes is the caller's to hold to its batch."""
+    if _whole_step and torch.cuda.is_current_stream_capturing():
+        raise RuntimeError(f"{name}: belongs to one batch; training_step does not capture a step that uses it")

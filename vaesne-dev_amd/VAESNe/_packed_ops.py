@@ -15,7 +15,7 @@ import numpy as np
 import torch
 from torch.autograd.function import once_differentiable
 
-from . import _defer, _lib
+from . import _capture, _defer, _lib
 from ._lib import lib
 from ._ops import _rows
 
@@ -129,7 +129,8 @@ class PackedSequences:
 
     Make it once per batch (on the host: no synchronisation) and share it between layers.  It keeps
     device tables, so a captured graph that used it needs it alive; use it once before capturing,
-    since a table that is still missing cannot be copied to the device inside a capture."""
+    since a table that is still missing cannot be copied to the device inside a capture.
+    training_step never captures a step that uses one: a replay would keep its first batch's lengths."""
 
     def __init__(self, lengths, key_lengths=None, device="cuda"):
         self.lengths = _lengths(lengths, "lengths")
@@ -173,6 +174,7 @@ class PackedSequences:
         """from_mask's places and shape; the places are noted on the stream that will read them."""
         if self._index is None:
             raise RuntimeError(f"PackedSequences.{name}: only for sequences made by from_mask")
+        _capture.refuse_in_step("PackedSequences")
         self._index[0].record_stream(torch.cuda.current_stream(self.device))
         return self._index
 
@@ -234,6 +236,7 @@ class PackedSequences:
 
     def _args(self, call):
         """A fresh argument struct of `call`; the tables are noted on the stream that will read them."""
+        _capture.refuse_in_step("PackedSequences")
         raw = torch._C._cuda_getCurrentRawStream(self.device.index)
         for t, stream in call[2]:
             if stream != raw:

@@ -19,7 +19,9 @@ batches + its ragged last batch).  A signature is captured after WARMUP eager
 batches; a capture that fails (a loss function that synchronises, say) marks the
 signature eager for good.
 
-Not captured (always eager): injected or torch-CPU-generator noise
+Not captured (always eager): a step that uses PackedSequences (they belong to one batch,
+and a replay would keep the first batch's; found on a module, in the loss function's
+closure, defaults or globals, or refused by the call inside the capture); injected or torch-CPU-generator noise
 (rng.inject_uniform / rng.set_mode("torch_cpu"): the parity paths), host tensors,
 VAESNE_STEP_GRAPH=0.  Randomness: training_step restarts the RNG call ids at every
 batch and advances the device counter after it, so a replayed batch draws exactly
@@ -36,6 +38,8 @@ import torch
 
 from . import _config, _defer, rng, training_util
 from ._capture import guarded as _guarded
+from ._capture import whole_step as _whole_step
+from ._packed_ops import PackedSequences
 
 WARMUP = 2
 MAX_GRAPHS = 3
@@ -47,7 +51,8 @@ def _scalar_key(v, depth=0):
     """The value key of a number (Python or numpy: an llik_scaling of 1/np.float64(beta)),
     string, None or a tuple / list of them; a tensor by its storage, shape and dtype (a
     graph reads the memory it was captured on, so re-binding the attribute to another
-    tensor is a new signature while in-place updates need none); _SKIP otherwise."""
+    tensor is a new signature while in-place updates need none); a PackedSequences by
+    itself; _SKIP otherwise."""
     if v is None or isinstance(v, (str, bool)):
         return v
     if isinstance(v, numbers.Number):
@@ -56,6 +61,8 @@ def _scalar_key(v, depth=0):
         return (type(v).__name__, v)
     if isinstance(v, torch.Tensor):
         return ("tensor", v.data_ptr(), tuple(v.shape), v.dtype, v.device)
+    if isinstance(v, PackedSequences):
+        return v
     if isinstance(v, (tuple, list)) and depth < 2 and len(v) <= 16:
         ks = tuple(_scalar_key(e, depth + 1) for e in v)
         return _SKIP if any(k is _SKIP for k in ks) else (type(v).__name__,) + ks
@@ -74,9 +81,34 @@ _CACHE: "weakref.WeakKeyDictionary" = weakref.WeakKeyDictionary()
 _warned = set()
 
 
+def _plans(v, depth=0):
+    """The PackedSequences that `v` is or, as a container, holds."""
+    if isinstance(v, PackedSequences):
+        return (v,)
+    if depth < 3 and isinstance(v, (tuple, list, dict)) and len(v) <= 64:
+        return sum((_plans(e, depth + 1) for e in (v.values() if isinstance(v, dict) else v)), ())
+    return ()
+
+
+def _fn_plans(fn):
+    """The PackedSequences that a function finds in its closure, defaults or globals."""
+    code = getattr(fn, "__code__", None)
+    if code is None:
+        return ()
+    found = [c.cell_contents for c in (fn.__closure__ or ())] + list(fn.__defaults__ or ())
+    found += list((fn.__kwdefaults__ or {}).values())
+    g = getattr(fn, "__globals__", {})
+    found += [g[n] for n in code.co_names if n in g]
+    return sum(map(_plans, found), ())
+
+
 def _value_key(v):
     """Numbers, strings, tensors and tuples of them by value (_scalar_key); anything
-    else (functions, modules, containers) by identity."""
+    else (functions, modules, containers) by identity.  PackedSequences, and containers
+    of them, are one key whatever they are: ranks meet when this key is new (_fn_plans
+    tells them apart)."""
+    if _plans(v):
+        return ("packed", type(v).__name__)
     k = _scalar_key(v)
     return ("id", id(v)) if k is _SKIP else k
 
@@ -89,7 +121,7 @@ def _fn_key(fn):
     g = getattr(fn, "__globals__", {})
     names = []
     for n in code.co_names:     # the scalar globals it names (a script's K, beta, ...)
-        if n in g:
+        if n in g and not _plans(g[n]):
             k = _scalar_key(g[n])
             if k is not _SKIP:
                 names.append((n, k))
@@ -114,8 +146,12 @@ def _walk(network):
     if w is not None and _walk_valid(w):
         return w[0], w[1]
     scalars, params, mods = _walk_full(network)
-    _WALKS[network] = (scalars, params, mods)
+    _WALKS[network] = (scalars, params, mods, _holds_plan(scalars))
     return scalars, params
+
+
+def _holds_plan(key):
+    return isinstance(key, PackedSequences) or (isinstance(key, tuple) and any(map(_holds_plan, key)))
 
 
 def _walk_valid(w):
@@ -193,7 +229,13 @@ def _signature(network, loss_fn, xs, multimodal, params, scalars=None):
     if scalars is None:
         scalars = _module_scalars(network)
     return (_fn_key(loss_fn), multimodal, tuple((tuple(t.shape), t.dtype) for t in xs),
-            tuple((p.data_ptr(), p.requires_grad) for p in params), scalars)
+            tuple((p.data_ptr(), p.requires_grad) for p in params), scalars, _fn_plans(loss_fn))
+
+
+def _uses_plan(network, loss_fn):
+    """Whether a step of these uses PackedSequences, as far as they are found."""
+    _walk(network)
+    return _WALKS[network][3] or bool(_fn_plans(loss_fn))
 
 
 def step(network, loss_fn, x, multimodal):
@@ -205,6 +247,8 @@ def step(network, loss_fn, x, multimodal):
     if not all(t.is_cuda for t in xs):
         return None
     scalars, params = _walk(network)
+    if _WALKS[network][3] or _fn_plans(loss_fn):
+        return None
     key = _signature(network, loss_fn, xs, multimodal, params, scalars)
     graphs = _CACHE.setdefault(network, {})
     ent = graphs.get(key)
@@ -250,7 +294,7 @@ def _capture(ent, network, loss_fn, x, xs, multimodal, params) -> bool:
     try:
         torch.cuda.synchronize()
         with torch.cuda.graph(g):
-            with _guarded(), _defer.deferred():
+            with _guarded(), _whole_step(), _defer.deferred():
                 sloss = training_util.backward_negated(loss_fn(network, sx), negate=False)
     except Exception as e:   # noqa: BLE001 -- any capture failure: this signature stays eager
         ent.failed = True
