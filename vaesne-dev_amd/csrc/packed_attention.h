@@ -68,7 +68,6 @@ struct Args {
   float* part_lse;             // [split_q][rows]
   float* delta;                // [total_q][Hq]: rowsum(dO O)
   float* hist;                 // [dQ workgroups][2R + 1]
-  float *wgmax, *domax;        // fp16: max |dO| of delta_kernel's workgroups, of each key head [Hkv]
 };
 
 __device__ __forceinline__ int div_pg(const Args& a, int row) {
@@ -558,17 +557,47 @@ __global__ __launch_bounds__(256) void join_kernel(const float* part, const floa
 // -------------------------------------------------------------------------------------------
 // backward: dQ (and rowsum(dO O), the bias sums by relative position)
 // -------------------------------------------------------------------------------------------
-// fp16 has few exponents: dS enters the products scaled by a power of two taken from |dO|, 2^-e with
-// max |dO| in [2^e, 2^(e+1)), times 2^-3 (|dP| < 2^-2 sum |v|); it is taken out of the fp32 results.
-// bf16 and fp32 have fp32's range and take 1.
-__device__ __forceinline__ float pow2_of(uint32_t bits) {   // 2^e of |x|, 1 for 0 / inf / NaN
-  const uint32_t e = bits >> 23;
-  return e == 0 || e >= 255 ? 1.f : __uint_as_float(e << 23);
+// fp16 has few exponents, so its dS enters the products times a power of two that is taken out of the fp32
+// results.  Each column (a query's dQ, a key's dK) has its own, from the largest |dS| it has met: that one
+// lies in [2^12, 2^13) when the power is chosen, and a larger one may come up to 2^15 before the power is
+// chosen again and the sums so far are scaled to it (exact; a tile or two of a walk).  Nothing of another row,
+// sequence or batch enters, no size of dO or v overflows, and of the second part 2^-37 of the column's largest dS is
+// lost at most, however many keys share the row.  (One power for a whole batch from max |dO|, with room for |v| of 2^18,
+// left nothing of the second part from 65536 keys on, or beside a sequence of larger gradients.)
+// bf16 and fp32 have fp32's range and take 1.  Measured, training with 12 heads of 64: 113 us for the launch with the
+// batch's power, 121 so, without the launch of 2.4 us that found max |dO|.
+struct Power {
+  float up = 1.f, down = 1.f, most = 0x1p-100f;   // 1 / the power, the power, the |dS| up to which it stays (below 2^-100: nothing)
+  // chosen again for this lane's largest |dS|: what the sums so far are multiplied by
+  __device__ __forceinline__ float choose(float big) {
+    if (!(big > most)) return 1.f;
+    const uint32_t e = min(__float_as_uint(big) >> 23, 254u);      // (an infinity: its column is lost anyway)
+    const float p = __uint_as_float(e << 23), old = up;
+    up = p * 0x1p-12f;
+    down = 1.f / up;
+    most = p * 8.f;
+    return old * down;
+  }
+};
+// one 32 x 32 tile of dS in fp32 -> times its columns' powers; acc: the sums so far
+template <int DT> __device__ __forceinline__ void fit(f16v& ds, Power& pw, f16v (&acc)[DT]) {
+  float big = fabsf(ds[0]);
+#pragma unroll
+  for (int r = 1; r < 16; ++r) big = fmaxf(big, fabsf(ds[r]));
+  if (__builtin_amdgcn_ballot_w64(big > pw.most) != 0) {
+    const float f = pw.choose(xmax32(big));        // (lanes l and l ^ 32 share a column)
+#pragma unroll
+    for (int i = 0; i < DT; ++i)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[i][r] *= f;
+  }
+#pragma unroll
+  for (int r = 0; r < 16; ++r) ds[r] *= pw.down;
 }
 
 // acc += X^T dS over the rows of contraction block t.  fp16's dS goes in two parts: rounded once it would be off
 // as much as the gradient's own rounding (1.5 roundings in all, so 1.1), and fp16 is chosen for its
-// digits (training, 12 heads of 64: the launch 102 -> 112 us).  bf16 keeps one part
+// digits (training, 12 heads of 64: the launch 102 -> 112 us, before the powers).  bf16 keeps one part
 // (10 k tokens, 16 heads of 128 over 4: two would take 910 us instead of 765).
 template <class L, class Lane> __device__ __forceinline__ void add_ds(f16v (&acc)[L::DT], const char* x, const Lane& at, int row0, int t, const f16v& ds) {
   using T = typename L::Type;
@@ -641,17 +670,7 @@ __device__ __forceinline__ void dq_body(const Args& a, int wg, int part_no) {
     for (int i = lane; i < SKEW; i += 64) skew[i] = 0.f;
   }
   const float lse = valid ? lse_in : INF;
-  float up = 1.f;                                              // 1 / (the factor on dS)
-  if (HALF) {
-    float big = 0.f;
-#pragma unroll
-    for (int k = 0; k < L::NCH; ++k)
-#pragma unroll
-      for (int e = 0; e < L::EPC; ++e) big = fmaxf(big, fabsf((float)gf[k][e]));
-    big = xmax32(big);
-    up = 8.f * pow2_of(__float_as_uint(big));
-  }
-  const float down = 1.f / up;
+  Power power;
   // dP starts from -delta where the registers allow a copy of it (one subtraction less per score)
   constexpr bool FROM = DP <= 64;
   f16v minus;
@@ -718,10 +737,7 @@ __device__ __forceinline__ void dq_body(const Args& a, int wg, int part_no) {
             *q += x;
           }
         }
-        if (HALF) {
-#pragma unroll
-          for (int r = 0; r < 16; ++r) s[r] *= down;
-        }
+        if (HALF) fit(s, power, o);
 #pragma unroll
         for (int b = 0; b < L::TB; ++b) {
           add_ds<L>(o, K, at, 32 * n, b, s);
@@ -762,7 +778,7 @@ __device__ __forceinline__ void dq_body(const Args& a, int wg, int part_no) {
     }
   }
   if (!valid) return;
-  const float f = a.p.scale * up;
+  const float f = a.p.scale * power.up;
   if (nsplit == 1) store_col(reinterpret_cast<T*>(a.p.dq) + rid * D, o, f, D, h);
   else store_col(a.part + ((int64_t)part_no * a.p.total_q * a.p.Hq + rid) * D, o, f, D, h);
 }
@@ -821,9 +837,7 @@ __device__ __forceinline__ void dkv_body(const Args& a, int wg, int part_no) {
   f16v dk[L::DT], dv[L::DT];
 #pragma unroll
   for (int i = 0; i < L::DT; ++i) dk[i] = dv[i] = f16v{};
-  float up = 1.f;
-  if (HALF) up = 8.f * pow2_of(__float_as_uint(a.domax[kvh]));
-  const float down = 1.f / up;
+  Power power;
 
   // rows (position * PK + head) that see any of the tile's keys, tile by tile, one head group after
   // the other: it = sub * ntq + row tile.  PK, the heads that share a row tile, is a power of two, so a
@@ -938,7 +952,8 @@ __device__ __forceinline__ void dkv_body(const Args& a, int wg, int part_no) {
         feed<L::NCH, VL ? 2 : 1, VL ? 2 : 3>();
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[n][r] *= HALF ? g[n][r] * down : g[n][r];
+        for (int r = 0; r < 16; ++r) s[n][r] *= g[n][r];
+        if (HALF) fit(s[n], power, dk);
 #pragma unroll
         for (int t = 0; t < L::TB; ++t) {
           add_ds<L>(dk, Q, at, 32 * n, t, s[n]);
@@ -956,16 +971,16 @@ __device__ __forceinline__ void dkv_body(const Args& a, int wg, int part_no) {
   if (!valid) return;
   const int64_t rid = (k0 + key) * a.p.Hkv + kvh, rows = a.p.total_k * a.p.Hkv;
   if (nsplit == 1) {
-    store_col(reinterpret_cast<T*>(a.p.dk) + rid * D, dk, a.p.scale * up, D, h);
+    store_col(reinterpret_cast<T*>(a.p.dk) + rid * D, dk, a.p.scale * power.up, D, h);
     store_col(reinterpret_cast<T*>(a.p.dv) + rid * D, dv, 1.f, D, h);
   } else {
-    store_col(a.part_k + ((int64_t)part_no * rows + rid) * D, dk, a.p.scale * up, D, h);
+    store_col(a.part_k + ((int64_t)part_no * rows + rid) * D, dk, a.p.scale * power.up, D, h);
     store_col(a.part_k + ((int64_t)(nsplit + part_no) * rows + rid) * D, dv, 1.f, D, h);
   }
 }
 
 // -------------------------------------------------------------------------------------------
-// backward: both in one launch.  They need nothing of each other but rowsum(dO O) and max |dO|, which
+// backward: both in one launch.  They need nothing of each other but rowsum(dO O), which
 // delta_kernel takes first, and share the chip to the end instead of each leaving it half empty (training with 12 heads of 64, up to
 // 2047 tokens, dS in one part: dQ 81 and dK / dV 70 us one after the other, 102 together; 10 k tokens, 16 heads of 128 over 4:
 // 818 and 765 us, 0.68 TFLOP counted as seven products: 0.89 PFLOP/s)
@@ -977,14 +992,10 @@ __global__ __launch_bounds__(NW * 64, (occ_bwd<T, DP, BIAS, NW>())) void bwd_ker
   else dq_body<T, DP, BIAS, NW>(a, (id - nk) % a.wgs_q, (id - nk) / a.wgs_q);
 }
 
-// delta[row] = sum dO O over the features, 16 lanes a row, 64 tokens of one head a workgroup; fp16: each
-// workgroup's max |dO| too, of which max_kernel takes a key head's.  (Straight into domax by atomics:
-// 45 us for 1300 workgroups and 12 heads, one cache line.)
+// delta[row] = sum dO O over the features, 16 lanes a row, 64 tokens of one head a workgroup
 template <class T> __global__ __launch_bounds__(256) void delta_kernel(Args a) {
   constexpr int EPC = 16 / sizeof(T);
-  constexpr bool HALF = __is_same(T, _Float16);
   const int head = blockIdx.y, l = threadIdx.x & 15, D = a.p.D;
-  float big = 0.f;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int64_t tok = (int64_t)blockIdx.x * 64 + i * 16 + (threadIdx.x >> 4);
@@ -999,10 +1010,7 @@ template <class T> __global__ __launch_bounds__(256) void delta_kernel(Args a) {
         const auto gv = *reinterpret_cast<const typename Ty<T>::Frag*>(g + d);
         const auto ov = *reinterpret_cast<const typename Ty<T>::Frag*>(o + d);
 #pragma unroll
-        for (int e = 0; e < EPC; ++e) {
-          x = fmaf((float)gv[e], (float)ov[e], x);
-          if (HALF) big = fmaxf(big, fabsf((float)gv[e]));
-        }
+        for (int e = 0; e < EPC; ++e) x = fmaf((float)gv[e], (float)ov[e], x);
       }
     }
     x += dpp_mov<0x128>(x);                                    // over the row's 16 lanes
@@ -1010,14 +1018,6 @@ template <class T> __global__ __launch_bounds__(256) void delta_kernel(Args a) {
     x += dpp_mov<0x4e>(x);
     x += dpp_mov<0xb1>(x);
     if (tok < a.p.total_q && l == 0) a.delta[tok * a.p.Hq + head] = x;
-  }
-  if (HALF) {
-    __shared__ float waves[4];
-    big = wave_max(big);
-    if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = big;
-    __syncthreads();
-    if (threadIdx.x == 0)
-      a.wgmax[(int64_t)head * gridDim.x + blockIdx.x] = fmaxf(fmaxf(waves[0], waves[1]), fmaxf(waves[2], waves[3]));
   }
 }
 
@@ -1054,9 +1054,6 @@ template <class T, int DP, bool BIAS> int fwd_dp(const Plan& p, hipStream_t s) {
   return 0;
 }
 
-// domax[head] = max of the n values of the head's group (0 for none)
-__global__ __launch_bounds__(256) void max_kernel(const float* wgmax, int64_t n, float* domax);
-
 template <class T, int DP, bool BIAS> int bwd_dp(const Plan& p, hipStream_t s) {
   const Args& a = p.a;
   constexpr int BQ = row_tile<T, DP>(), RB = Tile<T, DP>::RB;
@@ -1064,10 +1061,6 @@ template <class T, int DP, bool BIAS> int bwd_dp(const Plan& p, hipStream_t s) {
   const int64_t blocks = (a.p.total_q + 63) / 64;
   if (blocks > 0) {
     hipLaunchKernelGGL((delta_kernel<T>), dim3((unsigned)blocks, a.p.Hq), dim3(256), 0, s, a);
-    VAESNE_CHECK_LAUNCH();
-  }
-  if (__is_same(T, _Float16)) {
-    hipLaunchKernelGGL(max_kernel, dim3(a.p.Hkv), dim3(256), 0, s, a.wgmax, blocks * a.group, a.domax);
     VAESNE_CHECK_LAUNCH();
   }
   const size_t lds_q = 4 * BN * RB + (BIAS ? ((1 + nw) * span_of(R) + 3) / 4 * 16 : 0) + (BIAS && a.p.dtable ? nw * SKEW * 4 : 0);

@@ -17,16 +17,6 @@ template <> int run_bwd<float>(const Plan& p, hipStream_t s);
 template <> int run_bwd<__bf16>(const Plan& p, hipStream_t s);
 template <> int run_bwd<_Float16>(const Plan& p, hipStream_t s);
 
-__global__ __launch_bounds__(256) void max_kernel(const float* wgmax, int64_t n, float* domax) {
-  __shared__ float waves[4];
-  float x = 0.f;
-  for (int64_t i = threadIdx.x; i < n; i += 256) x = fmaxf(x, wgmax[blockIdx.x * n + i]);
-  x = wave_max(x);
-  if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = x;
-  __syncthreads();
-  if (threadIdx.x == 0) domax[blockIdx.x] = fmaxf(fmaxf(waves[0], waves[1]), fmaxf(waves[2], waves[3]));
-}
-
 __global__ __launch_bounds__(1024) void hist_sum_kernel(const float* hist, int n, int Hq, int NH, float* rel) {
   __shared__ float part[16][64];
   const int c = blockIdx.x * 64 + (threadIdx.x & 63), slice = threadIdx.x >> 6, head = blockIdx.y;
@@ -144,8 +134,7 @@ int make_plan(const vaesne_packed_attn* a, int backward, Plan* p) {
   return 0;
 }
 
-// the workspace: parts of the forward or dQ, their statistics | of dK / dV | rowsum(dO O) | bias sums |
-// max |dO|
+// the workspace: parts of the forward or dQ, their statistics | of dK / dV | rowsum(dO O) | bias sums
 int64_t carve(Plan* p, int backward) {
   Args& r = p->a;
   const vaesne_packed_attn& a = r.p;
@@ -164,9 +153,6 @@ int64_t carve(Plan* p, int backward) {
   r.delta = take(backward ? qrows * 4 : 0);
   r.hist = take(p->hist_bytes);
   take(bias ? (int64_t)a.Hq * NH * 4 : 0);                       // behind hist: its sums
-  const bool half = backward && a.type == 2;
-  r.domax = take(half ? (int64_t)a.Hkv * 4 : 0);
-  r.wgmax = take(half ? (a.total_q + 63) / 64 * a.Hq * 4 : 0);
   return used;
 }
 
