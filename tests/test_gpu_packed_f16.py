@@ -126,3 +126,16 @@ def test_large_values_leave_the_gradients_finite(D):
     for name in ("dq", "dk"):
         r = roundings(got[name], want[name])
         assert r <= 2 * ROUNDINGS[name], (name, r)
+
+
+@pytest.mark.parametrize("keys,D", [(2047, 64), (8192, 64), (65536, 128), (200000, 64)])
+def test_value_gradients_over_long_keys(keys, D):
+    """P is about 1 / keys: below fp16's normal range from 16384 keys on."""
+    g = gen(105)
+    m = 40
+    q, do = normal(g, m, 1, D, dtype=torch.float16), normal(g, m, 1, D, dtype=torch.float16, scale=64.0)
+    k, v = normal(g, keys, 1, D, dtype=torch.float16), normal(g, keys, 1, D, dtype=torch.float16)
+    got = run_attention(q, k, v, P().PackedSequences([m], [keys]), do)
+    want = formula(q, k, v, do, D ** -0.5)
+    r = roundings(got["dv"], want["dv"])
+    assert r <= ROUNDINGS["dv"], r

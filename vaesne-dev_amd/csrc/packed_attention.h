@@ -838,6 +838,10 @@ __device__ __forceinline__ void dkv_body(const Args& a, int wg, int part_no) {
 #pragma unroll
   for (int i = 0; i < L::DT; ++i) dk[i] = dv[i] = f16v{};
   Power power;
+  // fp16's P enters dV times 2^14 (at most 2^14 but for the rounding of scores: below 65504): over 16384 keys
+  // and more P itself lies below the type's normal range (dV 10 roundings off at 200000 keys, so 1.4).  dS carries it too;
+  // both are taken out at the end.
+  constexpr float LIFT = HALF ? 14.f : 0.f, UNLIFT = HALF ? 0x1p-14f : 1.f;
 
   // rows (position * PK + head) that see any of the tile's keys, tile by tile, one head group after
   // the other: it = sub * ntq + row tile.  PK, the heads that share a row tile, is a power of two, so a
@@ -876,7 +880,7 @@ __device__ __forceinline__ void dkv_body(const Args& a, int wg, int part_no) {
     qs.store(smem + b * 2 * TILE);
     gs.store(smem + b * 2 * TILE + TILE);
     if (threadIdx.x < BQ) {
-      stat[b * 2 * BQ + threadIdx.x] = st_in ? st_l : INF;
+      stat[b * 2 * BQ + threadIdx.x] = st_in ? st_l - LIFT : INF;
       stat[b * 2 * BQ + BQ + threadIdx.x] = -st_d;
     }
   };
@@ -971,11 +975,11 @@ __device__ __forceinline__ void dkv_body(const Args& a, int wg, int part_no) {
   if (!valid) return;
   const int64_t rid = (k0 + key) * a.p.Hkv + kvh, rows = a.p.total_k * a.p.Hkv;
   if (nsplit == 1) {
-    store_col(reinterpret_cast<T*>(a.p.dk) + rid * D, dk, a.p.scale * power.up, D, h);
-    store_col(reinterpret_cast<T*>(a.p.dv) + rid * D, dv, 1.f, D, h);
+    store_col(reinterpret_cast<T*>(a.p.dk) + rid * D, dk, a.p.scale * power.up * UNLIFT, D, h);
+    store_col(reinterpret_cast<T*>(a.p.dv) + rid * D, dv, UNLIFT, D, h);
   } else {
-    store_col(a.part_k + ((int64_t)part_no * rows + rid) * D, dk, a.p.scale * power.up, D, h);
-    store_col(a.part_k + ((int64_t)(nsplit + part_no) * rows + rid) * D, dv, 1.f, D, h);
+    store_col(a.part_k + ((int64_t)part_no * rows + rid) * D, dk, a.p.scale * power.up * UNLIFT, D, h);
+    store_col(a.part_k + ((int64_t)(nsplit + part_no) * rows + rid) * D, dv, UNLIFT, D, h);
   }
 }
 
