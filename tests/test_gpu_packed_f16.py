@@ -139,3 +139,22 @@ def test_value_gradients_over_long_keys(keys, D):
     want = formula(q, k, v, do, D ** -0.5)
     r = roundings(got["dv"], want["dv"])
     assert r <= ROUNDINGS["dv"], r
+
+
+@pytest.mark.parametrize("keys,sink", [(16384, 14.0625), (65536, 17.0625), (131072, 17.0625)])
+def test_many_keys_far_below_the_largest_score(keys, sink):
+    """The first key's score (in powers of two) lies `sink` above all others', which together still hold
+    a good part of the sum.  Their P are equal, so its rounding does not average out: one rounding (2^-11) of their
+    share at most.  The mean over all results leaves little of the rounding of o itself (rms 2^-11 / 2 over 64 values of
+    each row): 2^-13.  (So many rows that the parts' workspace keeps the keys in one walk.)"""
+    D, rows = 64, 1 << 17
+    q = torch.zeros(rows, 8, D, dtype=torch.float16, device="cuda")
+    q[:, :, 0] = 1.0
+    k = torch.zeros(keys, 1, D, dtype=torch.float16, device="cuda")
+    k[0, :, 0] = sink
+    v = normal(gen(106), keys, 1, D, dtype=torch.float16, mean=2.0, scale=0.1)
+    scale = math.log(2.0)
+    got = P().packed_attention(q, k, v, P().PackedSequences([rows], [keys]), scale=scale)[:2, :1]
+    want = formula(q[:2, :1], k, v, torch.zeros_like(q[:2, :1]), scale)["o"]
+    off = (got.double() / want - 1).mean().abs().item() * 2.0 ** 11
+    assert off <= 1.25, off

@@ -88,7 +88,7 @@ __device__ __forceinline__ f16v mma(f4 a, f4 b, f16v c) {
 }
 
 // accumulator registers of contraction block t as the other operand's fragment.  16-bit types
-// round to nearest even here: P <= 2^8 and dS enter the matrix cores in the inputs' own type, the
+// round to nearest even here: P <= 2^8 (fp16 2^15) and dS enter the matrix cores in the inputs' own type, the
 // sums stay fp32 (a relative 2^-8 (bf16), 2^-11 (fp16) of each term at most, independent between terms)
 template <class T> __device__ __forceinline__ typename Ty<T>::Frag take(const f16v& s, int t) {
   constexpr int N = 16 / sizeof(T);
@@ -434,13 +434,16 @@ __global__ __launch_bounds__(NW * 64, (occ_fwd<T, DP, NW>())) void fwd_kernel(Ar
         for (int r = 0; r < 16; ++r) mt = fmaxf(mt, s[n][r]);
       mt = xmax32(mt);
       // the origin moves when the first key is seen, and only when a score exceeds it by 2^8 after that:
-      // exp2 stays <= 2^8, the sums are fp32
-      if (__any(mt > 8.f || (m == -INF && mt > -INF))) {
+      // exp2 stays <= 2^8, the sums are fp32.  fp16: it lies 2^7 below the largest score and moves at 2^15, so that P
+      // is a normal number down to 2^-21 of the largest (with the origin at the largest, down to 2^-14: 131072 keys
+      // 2^-17 below one took o 0.18 percent off)
+      constexpr float BELOW = __is_same(T, _Float16) ? 7.f : 0.f, ROOM = __is_same(T, _Float16) ? 15.f : 8.f;
+      if (__any(mt > ROOM || (m == -INF && mt > -INF))) {
         const bool first = m == -INF;
-        const float up = first ? mt : fmaxf(mt, 0.f);             // from the old origin (0 at first)
+        const float up = first ? mt - BELOW : fmaxf(mt - BELOW, 0.f);    // from the old origin (0 at first)
         const float f = first ? 0.f : __builtin_amdgcn_exp2f(-up);
         const float by = up == -INF ? 0.f : up;
-        m = first ? mt : m + up;
+        m = first ? up : m + up;
         l *= f;
 #pragma unroll
         for (int i = 0; i < L::DT; ++i)
