@@ -10,6 +10,7 @@ The operators stand by themselves too: packed_attention, gated_norm, pre_norm, g
 unpack8.  The padded layers of util_layers (fp32, key padding masks, dropout) are unchanged;
 PackedSequences.from_mask takes one of their batches over.  Every call is a launch of a hand-written
 gfx950 kernel (include/vaesne_hip.h), but for the plain products of Linear layers; there is no CPU path.
+Derivatives are first-order and reverse-mode: a second one raises, and so does a tensor with a forward-mode tangent.
 """
 from __future__ import annotations
 

@@ -13,6 +13,7 @@ import math
 
 import numpy as np
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _capture, _defer, _lib
@@ -70,7 +71,12 @@ def _lib_call(name, device, *args):
 
 
 def _type_of(name, *ts):
-    """The C type of tensors that must share one type and one ROCm device."""
+    """The C type of tensors that must share one type and one ROCm device (and carry no tangent: where no
+    gradient is asked for the autograd function is passed by, and would lose it)."""
+    if forward_ad._current_level >= 0:
+        for t in ts:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise NotImplementedError(f"{name}: there is no forward-mode derivative")
     _lib.require_device(*ts)
     first = ts[0]
     if first.dtype not in TYPES:
