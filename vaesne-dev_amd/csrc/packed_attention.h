@@ -283,6 +283,13 @@ __device__ __forceinline__ void load_bias(const Args& a, float* lut, int head) {
 
 __device__ __forceinline__ int acc_row(int r, int h) { return 8 * (r >> 2) + 4 * h + (r & 3); }
 
+// the LDS accesses of this wave's lanes before and after stay in program order: the hardware keeps it within
+// a wave, this holds the compiler to it where lanes read what other lanes wrote (no instruction)
+__device__ __forceinline__ void wave_order() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local");
+  __builtin_amdgcn_wave_barrier();
+}
+
 // a value that is the same in every lane, told to the compiler (scalar registers and branches)
 __device__ __forceinline__ int uni(int x) { return __builtin_amdgcn_readfirstlane(x); }
 
@@ -726,18 +733,19 @@ __device__ __forceinline__ void dq_body(const Args& a, int wg, int part_no) {
             for (int r = 0; r < 16; ++r) far_hi += s[r];
           } else {
             // Row i's keys are written i places further left, so that a column holds one distance: lane d
-            // sums column d over the 32 rows and adds it to this wave's sums.  (A wave's LDS operations
-            // keep their order; places that no key reaches stay zero.  Adding each score atomically took
-            // 280 cycles for 32 of them: dQ 145 us instead of 81, fp16 training with 12 heads of 64.)
+            // sums column d over the 32 rows and adds it to this wave's sums.  (Places that no key
+            // reaches stay zero.  Adding each score atomically took 280 cycles for 32 of them: dQ 145 us instead of 81, fp16 training with 12 heads of 64.)
             float* p = skew + 63 * (lane & 31) + 4 * h + 31;
 #pragma unroll
             for (int r = 0; r < 16; ++r) p[acc_row(r, 0)] = s[r];
+            wave_order();
             float x = 0.f;
 #pragma unroll
             for (int i = 0; i < 32; ++i) x += skew[64 * i + lane];
             // column d: distance base - qfirst + d - 31; column 63 holds nothing
             float* q = hist + (lo + lane + R + MARGIN);
             *q += x;
+            wave_order();                                      // (the next tile writes the rows and adds to these sums)
           }
         }
         if (HALF) fit(s, power, o);
@@ -767,6 +775,7 @@ __device__ __forceinline__ void dq_body(const Args& a, int wg, int part_no) {
     }
     far_lo = wave_sum(far_lo);
     far_hi = wave_sum(far_hi);
+    wave_order();
     if (lane == 0) {
       hist[MARGIN] = far_lo;
       hist[2 * R + MARGIN] = far_hi;                           // (R >= 1: not the same place)
