@@ -293,17 +293,32 @@ __device__ __forceinline__ void wave_order() {
 // a value that is the same in every lane, told to the compiler (scalar registers and branches)
 __device__ __forceinline__ int uni(int x) { return __builtin_amdgcn_readfirstlane(x); }
 
+// A row of a tile table, held to the packed tensors: whatever a table that was overwritten or freed says, no access
+// leaves them (scalar operations, ten a workgroup).
+struct Where {
+  int q0, k0, nq, nk, first;
+  __device__ __forceinline__ Where(const Args& a, const int32_t* t, bool queries) {
+    auto in = [&](int i, int most) { return min(max(uni(t[i]), 0), most); };
+    const int Tq = (int)a.p.total_q, Tk = (int)a.p.total_k;
+    q0 = in(0, Tq);
+    k0 = in(1, Tk);
+    nq = in(2, min(Tq - q0, a.p.max_q));
+    nk = in(3, min(Tk - k0, a.p.max_k));
+    first = in(4, queries ? nq : nk);
+  }
+};
+
 // where a workgroup's query tile lies
 struct QTile {
   int pos0, nq, nk, npos, nrows, off, kvh, head0;
   int64_t q0, k0;
   __device__ __forceinline__ QTile(const Args& a, int tile, int hidx) {
-    const int32_t* t = a.p.q_tiles + 8 * (int64_t)tile;
-    q0 = uni(t[0]);
-    k0 = uni(t[1]);
-    nq = uni(t[2]);
-    nk = uni(t[3]);
-    pos0 = uni(t[4]);
+    const Where at(a, a.p.q_tiles + 8 * (int64_t)tile, true);
+    q0 = at.q0;
+    k0 = at.k0;
+    nq = at.nq;
+    nk = at.nk;
+    pos0 = at.first;
     off = nk - nq;
     npos = min(a.p.q_tile, nq - pos0);
     nrows = npos * a.pg;
@@ -371,7 +386,7 @@ __global__ __launch_bounds__(NW * 64, (occ_fwd<T, DP, NW>())) void fwd_kernel(Ar
   const int qfirst = t.pos0 + w * 32 + t.off, qabs = t.pos0 + dpos + t.off;   // (a bias: one head per tile, row = position)
   const bool active = w * 32 < t.nrows;
   const int wmin = uni(t.limit(a, w * 32)), wmax = active ? uni(t.limit(a, min(w * 32 + 31, t.nrows - 1))) : 0;
-  const int kend = uni(t.limit(a, t.nrows - 1));
+  const int kend = t.nrows > 0 ? uni(t.limit(a, t.nrows - 1)) : 0;
   const int nt = (kend + BN - 1) / BN, t0 = blockIdx.y * a.per_q, t1 = min(nt, t0 + a.per_q);
 
   f16v o[L::DT];
@@ -651,7 +666,7 @@ __device__ __forceinline__ void dq_body(const Args& a, int wg, int part_no) {
   const bool active = w * 32 < t.nrows;
   const int wmin = w * 32 + 31 < t.nrows ? uni(t.limit(a, w * 32)) : 0;
   const int wmax = active ? uni(t.limit(a, min(w * 32 + 31, t.nrows - 1))) : 0;
-  const int kend = uni(t.limit(a, t.nrows - 1));
+  const int kend = t.nrows > 0 ? uni(t.limit(a, t.nrows - 1)) : 0;
   const int nt = (kend + BN - 1) / BN, t0 = part_no * a.per_q, t1 = min(nt, t0 + a.per_q);
 
   const T* kb = reinterpret_cast<const T*>(a.p.k) + t.k0 * a.p.k_ts + t.kvh * a.p.k_hs;
@@ -826,9 +841,9 @@ __device__ __forceinline__ void dkv_body(const Args& a, int wg, int part_no) {
   float* lut = stat + 4 * BQ;
   char* vt = smem + 4 * TILE + 16 * BQ + (BIAS ? (span_of(a.p.max_distance) * 4 + 15) / 16 * 16 : 0);   // this tile's V (VL)
   const int kvh = wg % a.p.Hkv, tile = wg / a.p.Hkv, D = a.p.D, R = a.p.max_distance;
-  const int32_t* tl = a.p.k_tiles + 8 * (int64_t)tile;
-  const int64_t q0 = uni(tl[0]), k0 = uni(tl[1]);
-  const int nq = uni(tl[2]), nk = uni(tl[3]), key0 = uni(tl[4]), off = nk - nq;
+  const Where tl(a, a.p.k_tiles + 8 * (int64_t)tile, false);
+  const int64_t q0 = tl.q0, k0 = tl.k0;
+  const int nq = tl.nq, nk = tl.nk, key0 = tl.first, off = nk - nq;
   const int lane = threadIdx.x & 63, w = uni(threadIdx.x >> 6), h = lane >> 5;
   const int key = key0 + w * 32 + (lane & 31);
   const bool valid = key < nk;
