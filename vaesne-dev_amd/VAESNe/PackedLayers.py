@@ -70,7 +70,8 @@ def gelu8(x):
 
 def linear8(x, weight, bias=None, act=None):
     """act(x) weight^T + bias, act None or "gelu", with x kept for the backward pass in 8 bits: the
-    output is that of the exact x, the weight's gradient takes act(kept x)."""
+    output is that of the exact x, the weight's gradient takes act(kept x).  Inside autocast too the result has
+    the tensors' own type."""
     return _packed_ops.linear8(x, weight, bias, act)
 
 

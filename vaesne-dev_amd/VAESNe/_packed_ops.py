@@ -8,6 +8,7 @@ which are copied to the device when a shape of call first needs them.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 import math
 
@@ -626,6 +627,13 @@ def _gelu(x):
     return y
 
 
+def _own_type():
+    """Around the library products of linear8: autocast would give them another type than their tensors'."""
+    if torch.is_autocast_enabled("cuda"):
+        return torch.autocast("cuda", enabled=False)
+    return contextlib.nullcontext()
+
+
 class Linear8Fn(torch.autograd.Function):
     """act(x) W^T + b that keeps x in 8 bits: the products are the library's, the backward reads the
     kept x once for GELU'(x) and the weight gradient's operand."""
@@ -646,6 +654,11 @@ class Linear8Fn(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, do):
+        with _own_type():
+            return Linear8Fn.gradients(ctx, do)
+
+    @staticmethod
+    def gradients(ctx, do):
         codes, exps, W = ctx.saved_tensors
         g = do.reshape(-1, W.shape[0]).contiguous()
         need = ctx.needs_input_grad
@@ -670,6 +683,7 @@ def linear8(x, weight, bias=None, act=None):
         raise ValueError("linear8: act is None or 'gelu'")
     if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1] or (bias is not None and tuple(bias.shape) != (weight.shape[0],)):
         raise ValueError("linear8: x [.., in], weight [out, in], bias [out]")
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
-        return Linear8Fn.apply(x, weight, bias, act == "gelu")
-    return torch.nn.functional.linear(_gelu(x) if act else x, weight, bias)
+    with _own_type():
+        if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
+            return Linear8Fn.apply(x, weight, bias, act == "gelu")
+        return torch.nn.functional.linear(_gelu(x) if act else x, weight, bias)
