@@ -660,7 +660,7 @@ class Linear8Fn(torch.autograd.Function):
     @staticmethod
     def gradients(ctx, do):
         codes, exps, W = ctx.saved_tensors
-        g = do.reshape(-1, W.shape[0]).contiguous()
+        g = do.reshape(math.prod(ctx.shape[:-1]), W.shape[0]).contiguous()
         need = ctx.needs_input_grad
         dx = dW = db = None
         dy = torch.mm(g, W) if (need[0] or ctx.act) else None
