@@ -581,7 +581,7 @@ int vaesne_pack(const float* const* srcs, const int64_t* offs, const int64_t* ns
  *   S = scale q k^T + table[lut[clamp(j - i - (nk - nq), -R, R) + R], head]   (table: nullable)
  *   causal: key j is seen iff j <= i + nk - nq;  o = softmax(S) v, 0 where nothing is seen.
  * Query head h reads key head h / (Hq / Hkv).  type: 0 fp32, 1 bf16, 2 fp16 (every tensor but the
- * fp32 statistics has it).  D: a multiple of 8, at most 128.  total_q, total_k < 2^30.
+ * fp32 statistics has it).  D: a multiple of 8, at most 128.  total_q, total_k <= 2^30 - 64.
  * q_tiles / k_tiles [n][8]: one row for every tile of q_tile positions / k_tile keys of a sequence, in any
  * order (longest work first is fastest): {first query token, first key token, queries, keys of the
  * sequence, first position of the tile, 0, 0, 0}; vaesne_packed_attn_tiles gives q_tile and k_tile. */

@@ -23,6 +23,7 @@ from ._ops import _rows
 
 TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 KINDS = {"rms": 0, "layer": 1}
+MAX_TOKENS = (1 << 30) - 64                               # (csrc/packed_attention.hip's)
 
 
 def _fields(spec):
@@ -105,8 +106,8 @@ def _lengths(lengths, name):
     out = [int(n) for n in lengths]
     if any(n < 0 or n != m for n, m in zip(out, lengths)):
         raise ValueError(f"PackedSequences: {name} are whole numbers from 0 up")
-    if sum(out) >= 1 << 30:
-        raise ValueError(f"PackedSequences: {name} add up to 2^30 or more tokens")
+    if sum(out) > MAX_TOKENS:
+        raise ValueError(f"PackedSequences: {name} add up to more than 2^30 - 64 tokens")
     return out
 
 

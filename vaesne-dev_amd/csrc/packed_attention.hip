@@ -38,7 +38,7 @@ constexpr int CUS = 256;
 constexpr int MAX_SPLIT = 64;
 constexpr int64_t MAX_PART = 256 << 20;
 constexpr int64_t MAX_STRIDE = 1 << 21;  // elements: a tile of 128 rows spans less than 2^31 bytes
-constexpr int64_t MAX_TOKENS = 1 << 30;  // 4 threads of a launch each; an axis of a grid has fewer than 2^32
+constexpr int64_t MAX_TOKENS = (1 << 30) - 64;  // 4 threads of a launch each, 64 a workgroup; an axis of a grid has fewer than 2^32
 constexpr int64_t MAX_ROWS = 1 << 25; // rows of one sequence: 32-bit row arithmetic with room
 
 // Parts to cut the streamed axis into, in units of a tile (about 1.2 us).  Each of `wgs` workgroups walks
@@ -71,7 +71,7 @@ int64_t up16(int64_t n) { return (n + 15) & ~(int64_t)15; }
 bool sizes_ok(const vaesne_packed_attn* a) {
   return a && a->type >= 0 && a->type <= 2 && a->Hq > 0 && a->Hkv > 0 && a->Hq % a->Hkv == 0 && a->D > 0 &&
          a->D <= 128 && a->D % 8 == 0 && a->nseq >= 0 && a->max_q >= 0 && a->max_k >= 0 && a->total_q >= 0 &&
-         a->total_k >= 0 && a->total_q < MAX_TOKENS && a->total_k < MAX_TOKENS && a->scale > 0.f && a->Hq <= 4096 &&
+         a->total_k >= 0 && a->total_q <= MAX_TOKENS && a->total_k <= MAX_TOKENS && a->scale > 0.f && a->Hq <= 4096 &&
          (a->table == nullptr || (a->max_distance >= 1 && a->max_distance <= 512 && a->num_buckets >= 1));
 }
 
