@@ -578,7 +578,7 @@ int vaesne_pack(const float* const* srcs, const int64_t* offs, const int64_t* ns
  * Sequences of different lengths lie one behind the other, without padding: q [total_q, Hq, D],
  * k, v [total_k, Hkv, D] (rows of D unit-stride elements, 16-byte aligned; ts / hs = token / head
  * stride in elements).  A sequence's queries are the LAST nq of its nk positions (query i stands at i + nk - nq).
- *   S = scale q k^T + table[lut[clamp(j - i - (nk - nq), -R, R) + R], head]   (table: nullable)
+ *   S = scale q k^T + table[lut[clamp(j - i - (nk - nq), -R, R) + R], head]   (table: nullable; below -11356: masked)
  *   causal: key j is seen iff j <= i + nk - nq;  o = softmax(S) v, 0 where nothing is seen.
  * Query head h reads key head h / (Hq / Hkv).  type: 0 fp32, 1 bf16, 2 fp16 (every tensor but the
  * fp32 statistics has it).  D: a multiple of 8, at most 128.  total_q, total_k <= 2^30 - 64.

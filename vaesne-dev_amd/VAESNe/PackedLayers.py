@@ -34,7 +34,8 @@ def packed_attention(q, k, v, seqs, causal=False, scale=None, bias=None, buckets
     seqs: the PackedSequences of q and k.  A sequence's queries are the last positions of its keys,
     so with `causal` query i sees keys 0 .. i + (keys - queries); a query that sees none
     gives zeros and no gradient.  scale: default dim ** -0.5.  bias [buckets, heads] with `buckets`
-    (RelativeBuckets): bias[bucket(key position - query position), head] is added to the scaled score.
+    (RelativeBuckets): bias[bucket(key position - query position), head] is added to the scaled score; one below
+    -11356, as -inf, masks its keys.
     Gradients for q, k, v and bias; sums and softmax statistics in fp32; results are bitwise
     reproducible.  An infinity or NaN reaches queries and keys of its own sequence only (with `causal`,
     also earlier ones in it).  No dropout."""

@@ -269,7 +269,9 @@ __device__ __forceinline__ void store_col(U* p, const f16v (&o)[DT], float f, in
 
 // The bias of every relative position for one head, log2 domain: -R .. R and MARGIN more on either
 // side that repeat the ends, so that a tile which is not wholly beyond +-R reads without clamping.
+// A bias below LOWEST (log2 domain, -11356 in the table) masks, as -inf does: fp32 statistics could not hold the score beside it.
 constexpr int MARGIN = 64, SKEW = 2048;
+constexpr float LOWEST = -16384.f;
 __host__ __device__ __forceinline__ int span_of(int R) { return 2 * (R + MARGIN) + 1; }
 template <class T, int NT>
 __device__ __forceinline__ void load_bias(const Args& a, float* lut, int head) {
@@ -277,7 +279,8 @@ __device__ __forceinline__ void load_bias(const Args& a, float* lut, int head) {
   const int R = a.p.max_distance;
   for (int i = threadIdx.x; i < span_of(R); i += NT) {
     const int b = min(max(a.p.lut[min(max(i - MARGIN, 0), 2 * R)], 0), a.p.num_buckets - 1);
-    lut[i] = (float)tb[(int64_t)b * a.p.Hq + head] * LOG2E;
+    const float x = (float)tb[(int64_t)b * a.p.Hq + head] * LOG2E;
+    lut[i] = x < LOWEST ? -INF : x;
   }
 }
 
@@ -382,7 +385,6 @@ __global__ __launch_bounds__(NW * 64, (occ_fwd<T, DP, NW>())) void fwd_kernel(Ar
   const int row = w * 32 + (lane & 31), dpos = div_pg(a, row);
   const bool valid = row < t.nrows;
   const int head = t.head0 + row - dpos * a.pg;
-  const int lim = valid ? t.limit(a, row) : t.nk;
   const int qfirst = t.pos0 + w * 32 + t.off, qabs = t.pos0 + dpos + t.off;   // (a bias: one head per tile, row = position)
   const bool active = w * 32 < t.nrows;
   const int wmin = uni(t.limit(a, w * 32)), wmax = active ? uni(t.limit(a, min(w * 32 + 31, t.nrows - 1))) : 0;
@@ -392,7 +394,11 @@ __global__ __launch_bounds__(NW * 64, (occ_fwd<T, DP, NW>())) void fwd_kernel(Ar
   f16v o[L::DT];
 #pragma unroll
   for (int i = 0; i < L::DT; ++i) o[i] = f16v{};
-  float m = -INF, l = 0.f;
+  // the origin (0 until a key is seen) and the largest score beside it that leaves it where it is.  Behind keys that
+  // a bias puts far below, the origin is far below too, and a score on top of it would lose its digits: DEPTH of it at
+  // most are taken off at once (2^-18 of P), the rest once the tile's own largest score is known.
+  constexpr float BELOW = __is_same(T, _Float16) ? 7.f : 0.f, ROOM = __is_same(T, _Float16) ? 15.f : 8.f, DEPTH = BIAS ? 64.f : INF;
+  float m = 0.f, most = -INF, l = 0.f;
 
   const T* kb = reinterpret_cast<const T*>(a.p.k) + t.k0 * a.p.k_ts + t.kvh * a.p.k_hs;
   const T* vb = reinterpret_cast<const T*>(a.p.v) + t.k0 * a.p.v_ts + t.kvh * a.p.v_hs;
@@ -432,7 +438,7 @@ __global__ __launch_bounds__(NW * 64, (occ_fwd<T, DP, NW>())) void fwd_kernel(Ar
       }
       feed<NB * L::NCH, 1, 4>();
       // to the log2 domain, from the running origin m on: s c [+ bias] - m
-      const float from = m == -INF ? 0.f : -m;
+      const float from = BIAS ? fminf(-m, DEPTH) : -m;
 #pragma unroll
       for (int n = 0; n < NB; ++n) {
         if constexpr (BIAS) {
@@ -443,6 +449,10 @@ __global__ __launch_bounds__(NW * 64, (occ_fwd<T, DP, NW>())) void fwd_kernel(Ar
         }
       }
       if (base + BN > wmin) {
+        // (found again from the lane's number: it would take a register through the loop)
+        uint32_t all = ~0u;
+        asm volatile("" : "+v"(all));
+        const int lim = t.limit(a, w * 32 + (int)(__builtin_amdgcn_mbcnt_hi(all, __builtin_amdgcn_mbcnt_lo(all, 0u)) & 31));
 #pragma unroll
         for (int n = 0; n < NB; ++n)
 #pragma unroll
@@ -459,13 +469,15 @@ __global__ __launch_bounds__(NW * 64, (occ_fwd<T, DP, NW>())) void fwd_kernel(Ar
       // exp2 stays <= 2^8, the sums are fp32.  fp16: it lies 2^7 below the largest score and moves at 2^15, so that P
       // is a normal number down to 2^-21 of the largest (with the origin at the largest, down to 2^-14: 131072 keys
       // 2^-17 below one took o 0.18 percent off)
-      constexpr float BELOW = __is_same(T, _Float16) ? 7.f : 0.f, ROOM = __is_same(T, _Float16) ? 15.f : 8.f;
-      if (__any(mt > ROOM || (m == -INF && mt > -INF))) {
-        const bool first = m == -INF;
-        const float up = first ? mt - BELOW : fmaxf(mt - BELOW, 0.f);    // from the old origin (0 at first)
+      if (__builtin_amdgcn_ballot_w64(mt > most) != 0) {
+        const bool first = most == -INF && !(-m > DEPTH);
+        if (BIAS) mt += -m - from;
+        const float up = first ? mt - BELOW : fmaxf(mt - BELOW, 0.f);    // from the old origin
         const float f = first ? 0.f : __builtin_amdgcn_exp2f(-up);
-        const float by = up == -INF ? 0.f : up;
-        m = first ? up : m + up;
+        const bool none = up == -INF;
+        m = none ? 0.f : m + up;
+        const float by = none ? 0.f : BIAS ? m + from : up;
+        most = none || -m > DEPTH ? -INF : ROOM;
         l *= f;
 #pragma unroll
         for (int i = 0; i < L::DT; ++i)
@@ -491,7 +503,9 @@ __global__ __launch_bounds__(NW * 64, (occ_fwd<T, DP, NW>())) void fwd_kernel(Ar
 #pragma unroll
           for (int dt = 0; dt < L::DT; ++dt) o[dt] = mma(L::col(V, at, 32 * n, b, dt), pf, o[dt]);
         }
-      feed<NB * L::TB * L::DT, L::CR, 3>();
+      // (with a bias and 128 registers, three fragments ahead do not fit and each is waited for: 91.2 us for the sequences
+      // of 300 to 982 above, two 90.5)
+      feed<NB * L::TB * L::DT, L::CR, BIAS && occ_fwd<T, DP, NW>() == 4 ? 2 : 3>();
     }
     if (j + 1 < t1) {
       char* Kn = smem + (1 - buf.value) * 2 * TILE;
