@@ -78,3 +78,30 @@ def test_a_bias_that_masks_every_key_gives_zeros(t):
     for name in ("o", "dq", "dk", "dv"):
         a, b = got[name][:, 1].double(), plain[name][:, 0].double()
         assert (a - b).norm() <= once * b.norm(), name
+
+
+@pytest.mark.parametrize("t", TYPES, ids=str)
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("size", [30.0, 1000.0])
+def test_keys_that_score_far_below_come_first(t, D, size):
+    """The same without a bias: the first 100 keys point away from every query."""
+    g = gen(142)
+    n = 300
+    q, k, v, do = (normal(g, n, 2, D, dtype=torch.float32) for _ in range(4))
+    q[..., 0] = 8.0
+    k[..., 0] = 0.0
+    k[:100, :, 0] = -size * D ** 0.5
+    q, k, v, do = (x.to(t) for x in (q, k, v, do))
+    got = run_attention(q, k, v, P().PackedSequences([n]), do)
+    buckets = P().RelativeBuckets(2, 2, bidirectional=False)
+    want = window64(q, k, v, do, torch.zeros(2, 2, device="cuda"), buckets, [], False)
+    for name in ("o", "dq", "dk", "dv"):
+        rows = slice(100, n) if name in ("dk", "dv") else slice(0, n)      # (nothing reaches the first keys)
+        a, b = got[name][rows].double(), want[name][rows]
+        cols = slice(1, D) if name == "dq" else slice(0, D)                # (dq's first column is a sum of large terms)
+        a, b = a[..., cols], b[..., cols]
+        off = (a - b).norm()
+        if t == torch.float32:
+            assert off <= 60 * F * b.norm(), (name, (off / b.norm() / F).item())
+        else:
+            assert off <= (1.8 if t == torch.bfloat16 and name in ("dq", "dk") else 1.6) * (b.to(t).double() - b).norm(), name

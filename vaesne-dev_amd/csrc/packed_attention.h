@@ -395,9 +395,9 @@ __global__ __launch_bounds__(NW * 64, (occ_fwd<T, DP, NW>())) void fwd_kernel(Ar
 #pragma unroll
   for (int i = 0; i < L::DT; ++i) o[i] = f16v{};
   // the origin (0 until a key is seen) and the largest score beside it that leaves it where it is.  Behind keys that
-  // a bias puts far below, the origin is far below too, and a score on top of it would lose its digits: DEPTH of it at
+  // score far below (a bias puts them there), the origin is far below too, and a score on top of it would lose its digits: DEPTH of it at
   // most are taken off at once (2^-18 of P), the rest once the tile's own largest score is known.
-  constexpr float BELOW = __is_same(T, _Float16) ? 7.f : 0.f, ROOM = __is_same(T, _Float16) ? 15.f : 8.f, DEPTH = BIAS ? 64.f : INF;
+  constexpr float BELOW = __is_same(T, _Float16) ? 7.f : 0.f, ROOM = __is_same(T, _Float16) ? 15.f : 8.f, DEPTH = 64.f;
   float m = 0.f, most = -INF, l = 0.f;
 
   const T* kb = reinterpret_cast<const T*>(a.p.k) + t.k0 * a.p.k_ts + t.kvh * a.p.k_hs;
@@ -438,7 +438,7 @@ __global__ __launch_bounds__(NW * 64, (occ_fwd<T, DP, NW>())) void fwd_kernel(Ar
       }
       feed<NB * L::NCH, 1, 4>();
       // to the log2 domain, from the running origin m on: s c [+ bias] - m
-      const float from = BIAS ? fminf(-m, DEPTH) : -m;
+      const float from = fminf(-m, DEPTH);
 #pragma unroll
       for (int n = 0; n < NB; ++n) {
         if constexpr (BIAS) {
@@ -471,12 +471,12 @@ __global__ __launch_bounds__(NW * 64, (occ_fwd<T, DP, NW>())) void fwd_kernel(Ar
       // 2^-17 below one took o 0.18 percent off)
       if (__builtin_amdgcn_ballot_w64(mt > most) != 0) {
         const bool first = most == -INF && !(-m > DEPTH);
-        if (BIAS) mt += -m - from;
+        mt += -m - from;
         const float up = first ? mt - BELOW : fmaxf(mt - BELOW, 0.f);    // from the old origin
         const float f = first ? 0.f : __builtin_amdgcn_exp2f(-up);
         const bool none = up == -INF;
         m = none ? 0.f : m + up;
-        const float by = none ? 0.f : BIAS ? m + from : up;
+        const float by = none ? 0.f : m + from;
         most = none || -m > DEPTH ? -INF : ROOM;
         l *= f;
 #pragma unroll
