@@ -17,6 +17,14 @@ template <> int run_bwd<float>(const Plan& p, hipStream_t s);
 template <> int run_bwd<__bf16>(const Plan& p, hipStream_t s);
 template <> int run_bwd<_Float16>(const Plan& p, hipStream_t s);
 
+__global__ __launch_bounds__(256) void add_parts_kernel(const float* part, int parts, int64_t n, float* out) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= n) return;
+  float x = 0.f;
+  for (int k = 0; k < parts; ++k) x += part[k * n + i];
+  out[i] = x;
+}
+
 __global__ __launch_bounds__(1024) void hist_sum_kernel(const float* hist, int n, int Hq, int NH, float* rel) {
   __shared__ float part[16][64];
   const int c = blockIdx.x * 64 + (threadIdx.x & 63), slice = threadIdx.x >> 6, head = blockIdx.y;
@@ -36,6 +44,7 @@ namespace {
 
 constexpr int CUS = 256;
 constexpr int MAX_SPLIT = 64;
+constexpr int ROW_TILES = 12;          // of a part of row_kernel's walk: its parts cost 4 bytes a row (8 to 16 are alike, 38 us; one part 48)
 constexpr int64_t MAX_PART = 256 << 20;
 constexpr int64_t MAX_STRIDE = 1 << 21;  // elements: a tile of 128 rows spans less than 2^31 bytes
 constexpr int64_t MAX_TOKENS = (1 << 30) - 64;  // 4 threads of a launch each, 64 a workgroup; an axis of a grid has fewer than 2^32
@@ -130,11 +139,13 @@ int make_plan(const vaesne_packed_attn* a, int backward, Plan* p) {
   if (backward && ((int64_t)r.wgs_q * r.split_q + (int64_t)r.wgs_k * r.split_k) * p->nwk * 64 >= 1ll << 32)
     return (int)hipErrorInvalidValue;
   r.per_q = (int)((long_q + r.split_q - 1) / r.split_q);
+  r.split_r = (int)std::max<int64_t>(1, std::min<int64_t>({(long_q + ROW_TILES - 1) / ROW_TILES, MAX_SPLIT, MAX_PART / std::max<int64_t>(qrows * 4, 1)}));
+  r.per_r = (int)((long_q + r.split_r - 1) / r.split_r);
   r.per_k = (int)((long_k + r.split_k - 1) / r.split_k);
   return 0;
 }
 
-// the workspace: parts of the forward or dQ, their statistics | of dK / dV | rowsum(dO O) | bias sums
+// the workspace: parts of the forward or dQ, their statistics | of dK / dV | rowsum(dO O) and its parts | bias sums
 int64_t carve(Plan* p, int backward) {
   Args& r = p->a;
   const vaesne_packed_attn& a = r.p;
@@ -151,6 +162,7 @@ int64_t carve(Plan* p, int backward) {
   r.part_lse = take(!backward && r.split_q > 1 ? r.split_q * qrows * 4 : 0);
   r.part_k = take(backward && r.split_k > 1 ? 2 * r.split_k * krows * a.D * 4 : 0);
   r.delta = take(backward ? qrows * 4 : 0);
+  r.part_delta = take(bias && a.type == 1 && r.split_r > 1 ? r.split_r * qrows * 4 : 0);
   r.hist = take(p->hist_bytes);
   take(bias ? (int64_t)a.Hq * NH * 4 : 0);                       // behind hist: its sums
   return used;
