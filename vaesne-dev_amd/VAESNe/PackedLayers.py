@@ -36,8 +36,10 @@ def packed_attention(q, k, v, seqs, causal=False, scale=None, bias=None, buckets
     gives zeros and no gradient.  scale: default dim ** -0.5.  bias [buckets, heads] with `buckets`
     (RelativeBuckets): bias[bucket(key position - query position), head] is added to the scaled score; one below
     -11356, as -inf, masks its keys.
-    Gradients for q, k, v and bias; sums and softmax statistics in fp32; results are bitwise
-    reproducible.  An infinity or NaN reaches queries and keys of its own sequence only (with `causal`,
+    Gradients for q, k, v and bias; results are bitwise reproducible.  Sums and softmax statistics are fp32; in
+    16-bit types the probabilities and (in the backward pass) their gradients are rounded to the type before their products
+    on the matrix cores, fp16's gradients in two parts, and rowsum(dout * out) takes the rounded output (bf16's bias
+    gradient: the probabilities).  An infinity or NaN reaches queries and keys of its own sequence only (with `causal`,
     also earlier ones in it).  No dropout."""
     return _packed_ops.packed_attention(q, k, v, seqs, causal, scale, bias, buckets)
 
@@ -113,8 +115,8 @@ class PackedTransformerBlock(nn.Module):
 
         a = out(attention(qkv(n)));  x, n = join1(x, a);  f = W2 gelu(W1 n);  x, n = join2(x, f)
 
-    The block takes the residual stream x and its norm n and returns the next pair, so a stack of blocks
-    reads every token once between two products.  `enter` is the norm before the first block."""
+    The block takes the residual stream x and its norm n and returns the next pair: one pass over the tokens
+    between out's product and the feed-forward, and between two blocks.  `enter` is the norm before the first block."""
 
     def __init__(self, embed_dim, num_heads, ff_dim, num_kv_heads=None, causal=False, buckets=None, kind="rms",
                  gate=None, residual_scale=1.0):

@@ -135,8 +135,8 @@ class PackedSequences:
     the same) of each, one behind the other.  A sequence's queries are the LAST ones of its keys'
     positions: one new token over a cache of n keys is lengths 1, key_lengths n.
 
-    Make it once per batch (on the host: no synchronisation) and share it between layers.  It keeps
-    device tables, so a captured graph that used it needs it alive; use it once before capturing,
+    Make it once per batch, on the host, and share it between layers; the first call that needs a table
+    copies it to the device and waits for the stream.  It keeps device tables, so a captured graph that used it needs it alive; use it once before capturing,
     since a table that is still missing cannot be copied to the device inside a capture.
     training_step never captures a step that uses one: a replay would keep its first batch's lengths."""
 

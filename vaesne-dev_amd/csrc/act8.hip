@@ -3,9 +3,9 @@
 // block's largest |x| is an integer maximum of bit patterns over the quad (two DPP moves), which also
 // finds infinities and NaN.  The step is a power of two, so scaling, rounding and reading back are
 // exact but for the one rounding to a whole code.  Bound by HBM: forward reads x and writes y, the
-// codes and 1/32 byte of exponents for each value (8192 x 16384 bf16: 675 MB either way, forward 0.124 ms,
-// backward 0.143 ms, 5.4 and 4.7 TB/s; a copy of 1 GiB reaches 5.2).  16 values per thread: 0.123 and
-// 0.173 ms; one ldexp per value in place of a product with the block's step: backward 0.160 ms.
+// codes and 1/32 byte of exponents for each value (8192 x 16384 bf16: 675 MB either way, forward 0.118 ms,
+// backward 0.134 ms, 5.7 and 5.0 TB/s; a copy of 1 GiB reaches 5.2).  16 values per thread: backward 0.173 ms instead of
+// 0.143; one ldexp per value in place of a product with the block's step: 0.160.
 #include "common.h"
 
 using namespace vaesne;

@@ -19,7 +19,7 @@
 // Measured (a product of 8192^3 reaches 1.2 PFLOP/s in bf16, 1.16 in fp16; a copy of 1 GiB 5.2 TB/s): three prompts
 // of 2000 to 8001 tokens, causal, 32 heads of 128 over 8, bf16, 0.74 TFLOP without the masked half: 0.75 ms, 0.98 PFLOP/s;
 // one new token over 32 caches, 0.43 GB of keys and values: 0.10 ms, 4.3 TB/s.  A kernel of many scores with a bias
-// at head_dim 64 is bound by the vector ALUs (exp2, the maximum, the bias read per score; 67 % busy).
+// at head_dim 64 spends most on the vector ALUs (exp2, the maximum, the bias read per score; 70 % busy).
 //
 // LDS tiles are rows of DP elements in 16-byte chunks, chunk c of row r at c ^ swz(r): both the row
 // reads (16 lanes: 16 rows of one chunk) and the transposed reads (32 lanes: 4 rows of 4 chunks)
