@@ -82,10 +82,11 @@ _warned = set()
 
 
 def _plans(v, depth=0):
-    """The PackedSequences that `v` is or, as a container, holds."""
+    """The PackedSequences that `v` is or, as a small container, holds (every batch looks; what it does not
+    find is refused by the call inside the capture)."""
     if isinstance(v, PackedSequences):
         return (v,)
-    if depth < 3 and isinstance(v, (tuple, list, dict)) and len(v) <= 64:
+    if depth < 2 and isinstance(v, (tuple, list, dict)) and len(v) <= 16:
         return sum((_plans(e, depth + 1) for e in (v.values() if isinstance(v, dict) else v)), ())
     return ()
 
