@@ -397,8 +397,8 @@ __global__ __launch_bounds__(NW * 64, (occ_fwd<T, DP, NW>())) void fwd_kernel(Ar
 #pragma unroll
   for (int i = 0; i < L::DT; ++i) o[i] = f16v{};
   // the origin (0 until a key is seen) and the largest score beside it that leaves it where it is.  Behind keys that
-  // score far below (a bias puts them there), the origin is far below too, and a score on top of it would lose its digits: DEPTH of it at
-  // most are taken off at once (2^-18 of P), the rest once the tile's own largest score is known.
+  // score far below (a bias puts them there), the origin is far below too, and a score on top of it would lose its
+  // digits: DEPTH of it at most are taken off at once (2^-18 of P), the rest once the tile's own largest score is known.
   constexpr float BELOW = __is_same(T, _Float16) ? 7.f : 0.f, ROOM = __is_same(T, _Float16) ? 15.f : 8.f, DEPTH = 64.f;
   float m = 0.f, most = -INF, l = 0.f;
 
@@ -474,10 +474,10 @@ __global__ __launch_bounds__(NW * 64, (occ_fwd<T, DP, NW>())) void fwd_kernel(Ar
       if (__builtin_amdgcn_ballot_w64(mt > most) != 0) {
         const bool first = most == -INF && !(-m > DEPTH);
         mt += -m - from;
-        const float up = first ? mt - BELOW : fmaxf(mt - BELOW, 0.f);    // from the old origin
-        const float f = first ? 0.f : __builtin_amdgcn_exp2f(-up);
+        const float up = first ? mt - BELOW : fmaxf(mt - BELOW, 0.f), old = m;
         const bool none = up == -INF;
         m = none ? 0.f : m + up;
+        const float f = first ? 0.f : __builtin_amdgcn_exp2f(old - m);   // (sums and scores move as far as m did, rounded)
         const float by = none ? 0.f : m + from;
         most = none || -m > DEPTH ? -INF : ROOM;
         l *= f;
@@ -765,7 +765,8 @@ __device__ __forceinline__ void dq_body(const Args& a, int wg, int part_no) {
           } else {
             // Row i's keys are written i places further left, so that a column holds one distance: lane d
             // sums column d over the 32 rows and adds it to this wave's sums.  (Places that no key
-            // reaches stay zero.  Adding each score atomically took 280 cycles for 32 of them: dQ 145 us instead of 81, fp16 training with 12 heads of 64.)
+            // reaches stay zero.  Adding each score atomically took 280 cycles for 32 of them: dQ 145 us
+            // instead of 81, fp16 training with 12 heads of 64.)
             float* p = skew + 63 * (lane & 31) + 4 * h + 31;
 #pragma unroll
             for (int r = 0; r < 16; ++r) p[acc_row(r, 0)] = s[r];
